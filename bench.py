@@ -9,7 +9,7 @@ the timed region starts.  One step = one forward of the batch through the native
 convolution launches, SPPF pooling, descriptor L2 norm, Detect decode to [8, 25200, 85]) replayed on the plan's two lanes.  N > 1: inference
 shards by independent images -- one replica per rank, no data-path collective, `scaling: weak`.
 
-Launch forms.  `python bench.py --gpus N` (no launcher around it) starts the N ranks itself: it re-executes as `python -m torch.distributed.run
+Launch forms.  `python bench.py --gpus N` (no launcher around it) starts the N ranks itself: it runs `python -m torch.distributed.run
 --nnodes=1 --nproc-per-node N --master-addr 127.0.0.1 --master-port <free> bench.py <same arguments>`, one rank per GPU over RCCL (the reference's
 `accelerate launch src/train.py`, README.md:76); under a launcher (WORLD_SIZE set -- the driver's form) it takes the launcher's ranks and exits with
 code 2 when `--gpus` disagrees with WORLD_SIZE or the box has fewer than N GPUs.  Rank 0 prints the ONE line (`n_gpus`: N).  `--backend gloo --dry`:
@@ -93,10 +93,11 @@ def parse():
 
 
 def self_launch(a, argv):
-    """`python bench.py --gpus N` with N > 1 and no launcher around it (WORLD_SIZE unset): become `torch.distributed.run --nnodes=1
+    """`python bench.py --gpus N` with N > 1 and no launcher around it (WORLD_SIZE unset): run `torch.distributed.run --nnodes=1
     --nproc-per-node N --master-addr 127.0.0.1 --master-port P bench.py <same arguments>` -- one rank per GPU, the form the reference is
-    started in (`accelerate launch src/train.py`, README.md:76; train.py:38-46,174).  The process image is replaced (exec), so rank 0's ONE
-    JSON line reaches this process's stdout unchanged.  Fails loudly when the box has fewer than N GPUs (never a silent N = 1 run)."""
+    started in (`accelerate launch src/train.py`, README.md:76; train.py:38-46,174), as a child process that inherits stdout (rank 0's ONE JSON
+    line passes unchanged) and whose exit code this process returns: counting the GPUs initialises the runtime, and such a process must not be
+    replaced by another program (exec is refused on the GPU machines).  Fails loudly when the box has fewer than N GPUs (never a silent N = 1 run)."""
     if not a.dry:
         have = torch.cuda.device_count() if torch.cuda.is_available() else 0
         if a.rehearsal and have < 1:
@@ -116,7 +117,9 @@ def self_launch(a, argv):
            "--master-port", port, os.path.abspath(__file__)] + list(argv)
     sys.stderr.write("bench.py: launching " + " ".join(cmd) + "\n")
     sys.stderr.flush()
-    os.execv(sys.executable, cmd)
+    import subprocess
+    rc = subprocess.call(cmd)
+    sys.exit(rc if rc >= 0 else 128 - rc)
 
 
 def dry_run(a, rank, world):
@@ -1056,7 +1059,7 @@ if __name__ == "__main__":
     sys.stdout.flush()
     _args = parse()
     if "WORLD_SIZE" not in os.environ and _args.gpus > 1:
-        self_launch(_args, sys.argv[1:])          # exec: does not return (before file descriptor 1 is redirected below)
+        self_launch(_args, sys.argv[1:])          # does not return (before file descriptor 1 is redirected below)
     _REAL_STDOUT_FD = os.dup(1)
     os.dup2(2, 1)           # everything else any library prints: stderr
     main(_args)
