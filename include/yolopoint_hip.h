@@ -665,6 +665,73 @@ int yp_mnn_match(const float* d1, int N1, const float* d2, int N2, int D, float 
                  size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------
+ * Operators on tokens: `rows` rows of D features (keypoint descriptors, cells of the descriptor map, entries of a sequence), for the
+ * transformer blocks that refine and match what the network extracts.  (no reference counterpart: the reference's network is convolutional and
+ * its matcher is models/model_wrap.py:434-476)
+ * dtype: YP_F16 | YP_BF16 | YP_F32; all sums, statistics and angles in 32 bits or more, results rounded once.  Rows may start on any element.
+ * ---------------------------------------------------------------------------------- */
+
+/* Layer norm, alone or behind dropout + residual.  One descriptor for both passes; strides are in elements between rows, the tensors the calls
+ * write are dense [rows][D].
+ *   forward   z = x, or with `res`: z = res + dropout(x), one fp32 multiply-add, rounded to dtype (written to `z`);
+ *             y = (z - mean) * rstd * weight + bias with mean / rstd of the stored z (weight NULL: 1, bias NULL: 0).
+ *             mean, rstd: fp32 [rows], both NULL when no backward pass follows.
+ *   backward  x = the z of the forward pass, mean / rstd as it wrote them, dy = gradient of y, dz = gradient of z (NULL: none).
+ *             dres = gradient of res (of x without a residual); dx = gradient of x, written where p > 0 only (it equals dres otherwise).
+ *             dweight, dbias in wdtype, each may be NULL; they need the workspace of yp_layer_norm_bwd_workspace_bytes (both NULL: none).
+ *             Two passes over the same inputs give the same bits.
+ *   dropout   rate p and the generator's state as in yp_dropout (element index = row * D + column).
+ *   wdtype    YP_F32 or dtype. */
+typedef struct YpLayerNormDesc {
+    const void *x, *res, *weight, *bias;
+    void *z, *y;
+    float *mean, *rstd;
+    const void *dy, *dz;
+    void *dres, *dx, *dweight, *dbias;
+    void* workspace;
+    const int64_t* rng;
+    int64_t rows, x_stride, res_stride, dy_stride, dz_stride;
+    uint64_t seed, offset;
+    size_t workspace_bytes;
+    double p;
+    float eps;
+    int32_t D;                       /* 1 .. yp_layer_norm_max_width(dtype) */
+    int32_t dtype, wdtype;
+} YpLayerNormDesc;
+int yp_layer_norm_max_width(int dtype);
+int yp_layer_norm_fwd(const YpLayerNormDesc* d, void* stream);
+size_t yp_layer_norm_bwd_workspace_bytes(int64_t rows, int D, int dtype);
+int yp_layer_norm_bwd(const YpLayerNormDesc* d, void* stream);
+
+/* Dropout [+ residual] over n dense elements: y = (res +) (kept ? x * scale : 0), the mask recomputed wherever it is needed and never stored (the
+ * gradient of x is the same call on the gradient).  Element i is kept where half i % 8 (low half of a word first) of Philox4x32-10 with the counter
+ * (i / 8 [64 bits], offset [64 bits]) and the key seed is >= t = round(65536 p); scale = 65536 / (65536 - t).  rng != NULL: seed and offset are read
+ * from rng[0], rng[1] on the device (a captured graph whose state advances between replays). */
+int yp_dropout(const void* x, const void* res, void* y, int64_t n, int dtype, double p, uint64_t seed, uint64_t offset, const int64_t* rng, void* stream);
+
+/* Rotary positions of B x T tokens with Hq (+ Hk) heads of D features: pair j < R / 2 of every head turns by positions * inv_freq[j] radians,
+ * (u, v) -> scale * (u cos - v sin, v cos + u sin); features R .. D - 1 are copied (left alone where an output is its input).
+ *   q, k      element (b, t, h, c) at b * stride[0] + t * stride[1] + h * stride[2] + c; outputs likewise (they may be the inputs themselves)
+ *   pairs     features (j, j + R / 2), or (2 j, 2 j + 1) when interleaved
+ *   positions of position_type, axis a of token (b, t) at b * position_stride[0] + t * position_stride[1] + a * position_stride[2]; NULL (one axis
+ *             only): start + t.  axes = 2: the first half of the pairs turns by axis 0, the second by axis 1 (keypoints at (x, y))
+ *   inv_freq  float64 [R / 2]; angles are formed and reduced in 64 bits
+ *   inverse   1: turn back (the gradient's direction) */
+enum { YP_POS_I32 = 0, YP_POS_I64 = 1, YP_POS_F32 = 2 };
+typedef struct YpRotaryDesc {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const void* positions;
+    const double* inv_freq;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3], position_stride[3];
+    int64_t start;
+    int32_t B, T, Hq, Hk, D, R;      /* B * T < 2^31, D <= 1024, R even */
+    int32_t dtype, position_type, axes, interleaved, inverse;
+    float scale;
+} YpRotaryDesc;
+int yp_rotary(const YpRotaryDesc* d, void* stream);
+
+/* ------------------------------------------------------------------------------------
  * Execution plan: an immutable, caller-owned list of the launches above, replayed with
  * one call (optionally through a captured hipGraph).  Buffers referenced by the
  * descriptors must stay alive and fixed for the life of the plan.

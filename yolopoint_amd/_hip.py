@@ -54,6 +54,22 @@ class YpOpArgs(C.Structure):
                 ("p", C.c_void_p * 2), ("n", C.c_size_t * 2), ("i", C.c_int32 * 8), ("s", C.c_float * 4)]
 
 
+class YpLayerNormDesc(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "res", "weight", "bias", "z", "y", "mean", "rstd", "dy", "dz", "dres", "dx", "dweight", "dbias", "workspace", "rng")]
+                + [(n, C.c_int64) for n in ("rows", "x_stride", "res_stride", "dy_stride", "dz_stride")]
+                + [("seed", C.c_uint64), ("offset", C.c_uint64), ("workspace_bytes", C.c_size_t), ("p", C.c_double), ("eps", C.c_float)]
+                + [(n, C.c_int32) for n in ("D", "dtype", "wdtype")])
+
+
+YP_POS_I32, YP_POS_I64, YP_POS_F32 = 0, 1, 2
+
+
+class YpRotaryDesc(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "positions", "inv_freq")]
+                + [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride", "position_stride")] + [("start", C.c_int64)]
+                + [(n, C.c_int32) for n in ("B", "T", "Hq", "Hk", "D", "R", "dtype", "position_type", "axes", "interleaved", "inverse")] + [("scale", C.c_float)])
+
+
 (OP_BN_STATS, OP_BN_APPLY, OP_BN_BWD, OP_UPS2_BWD, OP_ADD_VIEWS, OP_MAXPOOL5_BWD, OP_L2NORM_BWD, OP_DETECT_BWD_PACK, OP_TO_CHWB,
  OP_COL_SUM, OP_MEMSET0, OP_PACK_NCHW, OP_L2NORM, OP_SPPF_POOL, OP_CAST_F32, OP_MAXPOOL2, OP_PACK_WEIGHT, OP_WGRAD, OP_WGRAD_UNPACK, OP_MAXPOOL2_BWD, OP_WGRAD_UNPACK_BATCH, OP_WGRAD_GROUP,
  OP_SUM_SLABS, OP_STEM_WGRAD, OP_QUANT_FP8) = range(10, 35)
@@ -167,6 +183,12 @@ SIGNATURES = {
     "yp_desc_sample": (_i, [_p, _i, _i, _i, _i64, _i64, _i64, _p, _i, _i, _p, _p]),
     "yp_mnn_workspace_bytes": (_sz, [_i, _i]),
     "yp_mnn_match": (_i, [_p, _i, _p, _i, _i, _f, _p, _p, _i, _p, _sz, _p]),
+    "yp_layer_norm_max_width": (_i, [_i]),
+    "yp_layer_norm_fwd": (_i, [C.POINTER(YpLayerNormDesc), _p]),
+    "yp_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "yp_layer_norm_bwd": (_i, [C.POINTER(YpLayerNormDesc), _p]),
+    "yp_dropout": (_i, [_p, _p, _p, _i64, _i, C.c_double, C.c_uint64, C.c_uint64, _p, _p]),
+    "yp_rotary": (_i, [C.POINTER(YpRotaryDesc), _p]),
     "yp_plan_create": (_i, [C.POINTER(_p)]),
     "yp_plan_destroy": (_i, [_p]),
     "yp_plan_add_conv": (_i, [_p, C.POINTER(YpConvDesc)]),

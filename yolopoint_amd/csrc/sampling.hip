@@ -17,21 +17,6 @@
 
 namespace {
 
-struct U4 { unsigned x, y, z, w; };
-
-__device__ __forceinline__ U4 philox4x32(unsigned long long seed, unsigned long long ctr, unsigned stream) {
-    unsigned c0 = (unsigned)ctr, c1 = (unsigned)(ctr >> 32), c2 = stream, c3 = 0u;
-    unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const unsigned hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
-        const unsigned hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-        c0 = hi1 ^ c1 ^ k0; c1 = lo1; c2 = hi0 ^ c3 ^ k1; c3 = lo0;
-        k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
-    }
-    return U4{c0, c1, c2, c3};
-}
-
 __device__ __forceinline__ float lin11(int i, int n) {      // torch.linspace(-1, 1, n)[i]
     const float step = 2.0f / (float)(n - 1);
     return i < n / 2 ? -1.0f + step * (float)i : 1.0f - step * (float)(n - 1 - i);
@@ -104,7 +89,7 @@ __global__ __launch_bounds__(1024) void nce_select_kernel(const unsigned char* _
     if (b == 0 && t == 0) { meta[0] = pool; meta[1] = B * pool; meta[2] = 0; }
     if (pool <= 0) return;
     const unsigned char* vb = valid + (size_t)b * Nc;
-    for (int i = t; i < Nc; i += 1024) keys[i] = philox4x32(seed, (unsigned long long)b * Nc + i, 0u).x;
+    for (int i = t; i < Nc; i += 1024) keys[i] = yp_philox4x32(seed, (unsigned long long)b * Nc + i, 0u).x;
     __syncthreads();
     // ---- the pool-th smallest (key, cell) pair of the valid cells: binary search on the 48-bit value key << 16 | cell (pairs are distinct)
     unsigned long long lo = 0ull, hi = (1ull << 48) - 1ull;
@@ -154,7 +139,7 @@ __global__ __launch_bounds__(256) void nce_negatives_count_kernel(int n, int neg
     const size_t total = (size_t)n * negs;
     int c = 0;
     if (q * 4 < total) {
-        const U4 r = philox4x32(seed, q, 1u);
+        const YpU4 r = yp_philox4x32(seed, q, 1u);
         const unsigned rr[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -190,7 +175,7 @@ __global__ __launch_bounds__(256) void nce_negatives_write_kernel(int n, int neg
     }
     const size_t total = (size_t)n * negs;
     if (q * 4 >= total) return;
-    const U4 r = philox4x32(seed, q, 1u);
+    const YpU4 r = yp_philox4x32(seed, q, 1u);
     const unsigned rr[4] = {r.x, r.y, r.z, r.w};
     const float same = (float)meta[2];
 #pragma unroll
@@ -199,7 +184,7 @@ __global__ __launch_bounds__(256) void nce_negatives_write_kernel(int n, int neg
         if (e >= total) break;
         const int i = (int)(e / negs), j = (int)(e - (size_t)i * negs);
         int v = draw_row(rr[u], n);
-        if (v == i) v = (int)((float)(philox4x32(seed, e, 2u).x >> 8) * (1.0f / 16777216.0f) * same);
+        if (v == i) v = (int)((float)(yp_philox4x32(seed, e, 2u).x >> 8) * (1.0f / 16777216.0f) * same);
         idx[(size_t)i * E + 1 + j] = v;
         if (j == 0) idx[(size_t)i * E] = i;
     }

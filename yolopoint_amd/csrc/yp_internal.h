@@ -110,6 +110,21 @@ __device__ __forceinline__ void yp_block_amax(float mx, float* amax) {
     }
 }
 
+// Philox4x32-10 (Salmon et al., SC 2011): the four words of the 128-bit counter (ctr, stream) under a 64-bit key.
+struct YpU4 { unsigned x, y, z, w; };
+__device__ __forceinline__ YpU4 yp_philox4x32(unsigned long long seed, unsigned long long ctr, unsigned long long stream) {
+    unsigned c0 = (unsigned)ctr, c1 = (unsigned)(ctr >> 32), c2 = (unsigned)stream, c3 = (unsigned)(stream >> 32);
+    unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const unsigned hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
+        const unsigned hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
+        c0 = hi1 ^ c1 ^ k0; c1 = lo1; c2 = hi0 ^ c3 ^ k1; c3 = lo0;
+        k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
+    }
+    return YpU4{c0, c1, c2, c3};
+}
+
 // Thread t's sum of p[t], p[t + 256], p[t + 512], ... (i < n) in double precision, in that order, with eight loads in flight (the single-
 // workgroup folds behind the loss kernels walk 10-25 k partials: one dependent load per addition made them 13-25 us of pure latency).
 __device__ __forceinline__ double yp_strided_sum256(const float* __restrict__ p, int n) {
