@@ -1,0 +1,156 @@
+// Layer norm over the rows of a token tensor, forward: alone, or behind residual + dropout in the same pass.  Bound by HBM: a row is read once, stays in
+// registers while its statistics are formed, and is written once.
+#include "norm.h"
+
+namespace {
+
+struct LnFwd {
+    const void *x, *res, *weight, *bias;
+    void *z, *y;
+    float *mean, *rstd;
+    int64_t rows, xs, rs;
+    int D;
+    float eps;
+    bool w32;
+    unsigned long long seed, offset;
+    const int64_t* rng;
+    unsigned threshold;
+    float scale;
+};
+
+// mean = sum x / D;  var = sum (x - mean)^2 / D;  y = (x - mean) / sqrt(var + eps) w + b.  fp32 rows: delta = sum (x - mean) / D is what rounding left
+// of the mean, and is taken off as well (a row of mean 4096 and deviation 1 keeps 1e-7 instead of 1e-3; 16-bit rows have no such digits).
+// The next row is on its way while this one is worked on (the first before the weights are read).
+template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
+__global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
+    constexpr int N = Vec<T>::N, NC = E / N, ROWS = G ? 256 / G : 1;
+    constexpr bool FINE = sizeof(T) == 4;
+    __shared__ float2 sh[2][16];
+    const T *x = (const T*)a.x, *res = (const T*)a.res;
+    T *z = (T*)a.z, *y = (T*)a.y;
+    const int threads = G ? G : blockDim.x, t = G ? threadIdx.x % G : threadIdx.x;
+    const float inv_d = 1.0f / (float)a.D;
+    const Drop d = drop_state(a.seed, a.offset, a.rng, a.threshold, a.scale);
+    int c[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) c[k] = (t + k * threads) * N;
+    const int64_t first = (int64_t)blockIdx.x * ROWS + row_in_block<G>(), step = (int64_t)gridDim.x * ROWS;
+    Vec<T> nx[NC], nr[NC];
+    const T *px = x + min(first, a.rows - 1) * a.xs, *pr = RES ? res + min(first, a.rows - 1) * a.rs : nullptr;
+    auto fetch = [&]() {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            nx[k] = fetch_vec<T, TAIL>(px, c[k], a.D);
+            if constexpr (RES) nr[k] = fetch_vec<T, TAIL>(pr, c[k], a.D);
+        }
+    };
+    fetch();
+    float w[NC][N], b[NC][N];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) { load_weights<T, TAIL>(a.weight, a.w32, c[k], a.D, 1.f, w[k]); load_weights<T, TAIL>(a.bias, a.w32, c[k], a.D, 0.f, b[k]); }
+    for (int64_t row = first; row < a.rows; row += step) {
+        Vec<T> v[NC];
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            v[k] = settle<T, TAIL>(nx[k], c[k], a.D);
+            if constexpr (RES) {
+                const Vec<T> r = settle<T, TAIL>(nr[k], c[k], a.D), s = v[k];
+                drop_add<T, DROP>(d, (unsigned long long)row * a.D + c[k], s, r, v[k]);
+                store_vec<T, TAIL>(z + row * a.D, c[k], a.D, v[k]);
+            }
+        }
+        if (row + step < a.rows) {
+            px += step * a.xs;
+            if (RES) pr += step * a.rs;
+            fetch();
+        }
+        float f[NC][N], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) { f[k][j] = (float)v[k].e[j]; s1 += f[k][j]; }
+        const float mean = row_sum<G>(s1, sh[0]) * inv_d;
+        s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            const float m = c[k] < a.D ? mean : 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                f[k][j] -= m;
+                if constexpr (TAIL != WHOLE) f[k][j] = c[k] + j < a.D ? f[k][j] : 0.f;
+                if constexpr (FINE) s1 += f[k][j];
+                s2 = fmaf(f[k][j], f[k][j], s2);
+            }
+        }
+        if constexpr (FINE) row_sum2<G>(s1, s2, sh[1]);
+        else s2 = row_sum<G>(s2, sh[1]);
+        const float delta = FINE ? s1 * inv_d : 0.f;
+        float var = s2 * inv_d;
+        if constexpr (FINE) {
+            var = fmaf(-delta, delta, var);
+            var = var < 0.f ? 0.f : var;            // (not fmaxf: a NaN stays one)
+        }
+        const float rstd = rsqrtf(var + a.eps), shift = -delta * rstd;
+        if (a.mean != nullptr && t == 0) { a.mean[row] = mean + delta; a.rstd[row] = rstd; }
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            float o[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] = fmaf(FINE ? fmaf(f[k][j], rstd, shift) : f[k][j] * rstd, w[k][j], b[k][j]);
+            store_vec<T, TAIL>(y + row * a.D, c[k], a.D, to_vec<T>(o));
+        }
+    }
+}
+
+// The shape of a row: G threads with E features each, the first that holds it; G = 0: 64 * waves threads.  16 features a thread where 8 would need a
+// second wave (513 .. 1024 features: no barrier), or more than four.
+#define LN_SHAPES(X) X(4, 8) X(8, 8) X(16, 8) X(32, 8) X(64, 8) X(64, 16) X(0, 8) X(0, 16)
+struct LnShape { int G, E, threads; };
+LnShape ln_shape(int D) {
+#define PICK(G_, E_) if (G_ && D <= G_ * E_) return LnShape{G_, E_, G_};
+    LN_SHAPES(PICK)
+#undef PICK
+    const int E = D <= 2048 ? 8 : 16;
+    return LnShape{0, E, (D + 64 * E - 1) / (64 * E) * 64};
+}
+
+template <typename T> hipError_t ln_fwd_launch(const LnFwd& a, bool res, bool drop, hipStream_t st) {
+    const LnShape s = ln_shape(a.D);
+    const int block = s.G ? 256 : s.threads;
+    const int64_t per = s.G ? block / s.G : 1, want = (a.rows + per - 1) / per, most = 256 * 64 * 64 / block;     // (twice what the chip holds: the second half evens out)
+    const int blocks = (int)(want < most ? want : most);
+#define RUN(G_, E_, RES_, DROP_, TAIL_) do { ln_fwd_kernel<T, G_, E_, RES_, DROP_, TAIL_><<<blocks, block, 0, st>>>(a); return hipGetLastError(); } while (0)
+#define ENDS(G_, E_, RES_, DROP_) \
+    if (a.D % Vec<T>::N == 0) RUN(G_, E_, RES_, DROP_, WHOLE); \
+    else if (a.D > Vec<T>::N) RUN(G_, E_, RES_, DROP_, CUT); \
+    else if constexpr (G_ == 4) RUN(G_, E_, RES_, DROP_, SHORT);
+#define SHAPE(G_, E_) if (s.G == G_ && s.E == E_) { if (!res) { ENDS(G_, E_, false, false) } else if (!drop) { ENDS(G_, E_, true, false) } else { ENDS(G_, E_, true, true) } }
+    LN_SHAPES(SHAPE)
+#undef SHAPE
+#undef ENDS
+#undef RUN
+    return hipErrorInvalidValue;                    // (not reached: the shapes and row ends above are all there are)
+}
+
+}  // namespace
+
+extern "C" int yp_layer_norm_max_width(int dtype) { return dtype == YP_F16 || dtype == YP_BF16 || dtype == YP_F32 ? LN_WIDEST : 0; }
+
+extern "C" int yp_layer_norm_fwd(const YpLayerNormDesc* d, void* stream) {
+    YP_REQUIRE(d != nullptr, "yp_layer_norm_fwd: no descriptor");
+    YP_REQUIRE(ln_types(d), "yp_layer_norm_fwd: types %d / %d", d->dtype, d->wdtype);
+    YP_REQUIRE(d->rows >= 0 && d->D >= 1 && d->D <= LN_WIDEST, "yp_layer_norm_fwd: %lld rows of %d", (long long)d->rows, d->D);
+    if (d->rows == 0) return YP_OK;
+    YP_REQUIRE(d->x && d->y && (d->res == nullptr || d->z) && (d->mean == nullptr) == (d->rstd == nullptr), "yp_layer_norm_fwd: a buffer is missing");
+    YP_REQUIRE(d->x_stride >= 0 && d->res_stride >= 0, "yp_layer_norm_fwd: negative stride");
+    LnFwd a{};
+    YP_REQUIRE(drop_parameters(d->p, &a.threshold, &a.scale), "yp_layer_norm_fwd: a dropout rate of %g", d->p);
+    YP_REQUIRE(d->res != nullptr || a.threshold == 0, "yp_layer_norm_fwd: dropout needs a residual");
+    a.x = d->x; a.res = d->res; a.weight = d->weight; a.bias = d->bias; a.z = d->z; a.y = d->y; a.mean = d->mean; a.rstd = d->rstd;
+    a.rows = d->rows; a.xs = d->x_stride; a.rs = d->res_stride; a.D = d->D; a.eps = d->eps; a.w32 = d->wdtype == YP_F32;
+    a.seed = d->seed; a.offset = d->offset; a.rng = d->rng;
+    hipStream_t st = (hipStream_t)stream;
+    const bool res = d->res != nullptr, drop = a.threshold != 0;
+    YP_CHECK_HIP(d->dtype == YP_F16 ? ln_fwd_launch<_Float16>(a, res, drop, st) : d->dtype == YP_BF16 ? ln_fwd_launch<__bf16>(a, res, drop, st) : ln_fwd_launch<float>(a, res, drop, st));
+    return YP_OK;
+}

@@ -119,7 +119,8 @@ __device__ __forceinline__ YpU4 yp_philox4x32(unsigned long long seed, unsigned 
     for (int r = 0; r < 10; ++r) {
         const unsigned hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
         const unsigned hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-        c0 = hi1 ^ c1 ^ k0; c1 = lo1; c2 = hi0 ^ c3 ^ k1; c3 = lo0;
+        // (bitop3 0x96 = a ^ b ^ c in one instruction)
+        c0 = __builtin_amdgcn_bitop3_b32(hi1, c1, k0, 0x96); c1 = lo1; c2 = __builtin_amdgcn_bitop3_b32(hi0, c3, k1, 0x96); c3 = lo0;
         k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
     }
     return YpU4{c0, c1, c2, c3};
