@@ -15,6 +15,9 @@ template <int G> __device__ __forceinline__ int row_in_block() {
     return G ? threadIdx.x / G : 0;
 }
 
+// whether a thread is the last of its row's lanes in its wave
+template <int G> __device__ __forceinline__ bool last_lane() { return ((threadIdx.x + 1) & (G && G < 64 ? G - 1 : 63)) == 0; }
+
 // Sums over the threads of a row: G <= 64 neighbouring lanes, or (G = 0) `of` waves from wave `from` on (default: the workgroup's).  Calls alternate between
 // two areas of LDS, so that one barrier a call is enough: a wave writes an area again only behind the barrier of the call on the other one, which
 // every wave passes after reading the first.

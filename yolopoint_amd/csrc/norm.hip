@@ -55,7 +55,8 @@ __global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
             v[k] = settle<T, TAIL>(nx[k], c[k], a.D);
             if constexpr (RES) {
                 const Vec<T> r = settle<T, TAIL>(nr[k], c[k], a.D), s = v[k];
-                drop_add<T, DROP>(d, (unsigned long long)row * a.D + c[k], s, r, v[k]);
+                if (DROP && G == 0 && __ballot(c[k] < a.D) == 0ull) continue;       // (a wave behind the row's end makes no random numbers)
+                drop_add<T, DROP, TAIL != WHOLE, G == 0 || G == 64>(d, (unsigned long long)row * a.D + c[k], s, r, v[k], last_lane<G>(), a.D - c[k]);
                 store_vec<T, TAIL>(z + row * a.D, c[k], a.D, v[k]);
             }
         }

@@ -133,6 +133,7 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
         if (!real) continue;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
+            if (DROP && G == 0 && __ballot(c[k] < a.D) == 0ull) continue;           // (a wave behind the row's end makes no random numbers)
             const float sk = c[k] < a.D ? shift : 0.f;
             float o[N], wk[N];
             weights(k, wk);
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
             }
             Vec<T> ov;
             if constexpr (DROP) {
-                drop_only<T>(d, (unsigned long long)row * a.D + c[k], o, ov);
+                drop_only<T, TAIL != WHOLE, G == 0 || G == 64>(d, (unsigned long long)row * a.D + c[k], o, ov, last_lane<G>(), a.D - c[k]);
                 store_vec<T, TAIL>(dx + row * a.D, c[k], a.D, ov);
             }
             store_vec<T, TAIL>(dres + row * a.D, c[k], a.D, to_vec<T>(o));

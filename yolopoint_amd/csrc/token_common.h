@@ -190,31 +190,42 @@ __device__ __forceinline__ Drop drop_state(unsigned long long seed, unsigned lon
     return Drop{seed, offset, threshold, scale};
 }
 
-// the bits of N = 4 or 8 elements from flat index i on, two to a word
-template <int N> __device__ __forceinline__ void drop_bits(const Drop& d, unsigned long long i, unsigned (&w)[N / 2]) {
-    const unsigned sh = (unsigned)i & 7u;
+// The bits of N = 4 or 8 elements from flat index i on, two to a word.  STRADDLE: i may stand anywhere, so that the elements may need the next counter's
+// words too (rows of odd widths).  Those are what the next lane has just made of the counter after this one, so they come from there; `edge`: this
+// lane is the last of its row's lanes in the wave; `left`: elements of the row from i on.  A wave that holds one row (WAVE) makes the words of its last
+// lane's next counter on the scalar unit, beside the other waves' vector work.
+template <int N, bool STRADDLE, bool WAVE> __device__ __forceinline__ void drop_bits(const Drop& d, unsigned long long i, bool edge, int left, unsigned (&w)[N / 2]) {
+    const unsigned sh = WAVE && N == 8 ? __builtin_amdgcn_readfirstlane((unsigned)i & 7u) : (unsigned)i & 7u;       // (chunks of 8: the same for a row)
     const YpU4 a = yp_philox4x32(d.seed, i >> 3, d.offset);
-    if (N == 8 && sh == 0) {
-        w[0] = a.x; w[1] = a.y; w[N / 2 - 2] = a.z; w[N / 2 - 1] = a.w;
-        return;
-    }
-    if (N == 4 && (sh == 0 || sh == 4)) {
-        w[0] = sh ? a.z : a.x; w[1] = sh ? a.w : a.y;
-        return;
-    }
-    // the elements straddle two counters: shift the eight words right by sh halves
-    const YpU4 b = yp_philox4x32(d.seed, (i >> 3) + 1, d.offset);
-    unsigned v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    if (sh & 4) {
+    if constexpr (!STRADDLE) {                      // i % N == 0
+        if constexpr (N == 8) { w[0] = a.x; w[1] = a.y; w[N / 2 - 2] = a.z; w[N / 2 - 1] = a.w; }
+        else { w[0] = sh ? a.z : a.x; w[1] = sh ? a.w : a.y; }
+    } else {
+        auto from_next = [](unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x130, 0xf, 0xf, true); };     // (the wave shifted by a lane)
+        YpU4 b{from_next(a.x), from_next(a.y), from_next(a.z), from_next(a.w)};
+        if (__ballot(edge && left > 0 && (int)sh + min(N, left) > 8)) {
+            YpU4 s;
+            if constexpr (WAVE) {
+                const unsigned lo = __builtin_amdgcn_readlane((unsigned)(i >> 3), 63), hi = __builtin_amdgcn_readlane((unsigned)(i >> 35), 63);
+                s = yp_philox4x32<true>(d.seed, (((unsigned long long)hi << 32) | lo) + 1, d.offset);
+            } else {
+                s = yp_philox4x32(d.seed, (i >> 3) + 1, d.offset);
+            }
+            b.x = edge ? s.x : b.x; b.y = edge ? s.y : b.y; b.z = edge ? s.z : b.z; b.w = edge ? s.w : b.w;
+        }
+        // the eight words moved down by sh halves
+        unsigned v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        if (sh & 4) {
 #pragma unroll
-        for (int k = 0; k < 6; ++k) v[k] = v[k + 2];
-    }
-    if (sh & 2) {
+            for (int k = 0; k < 6; ++k) v[k] = v[k + 2];
+        }
+        if (sh & 2) {
 #pragma unroll
-        for (int k = 0; k < 7; ++k) v[k] = v[k + 1];
-    }
+            for (int k = 0; k < 7; ++k) v[k] = v[k + 1];
+        }
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) w[k] = (sh & 1) ? __builtin_amdgcn_alignbit(v[k + 1], v[k], 16) : v[k];
+        for (int k = 0; k < N / 2; ++k) w[k] = (sh & 1) ? __builtin_amdgcn_alignbit(v[k + 1], v[k], 16) : v[k];
+    }
 }
 
 template <int N> __device__ __forceinline__ bool drop_kept(const Drop& d, const unsigned (&w)[N / 2], int j) {
@@ -222,10 +233,11 @@ template <int N> __device__ __forceinline__ bool drop_kept(const Drop& d, const 
 }
 
 // out = res + (kept ? x * scale : 0): one fused multiply-add in fp32, rounded to T
-template <typename T, bool DROP> __device__ __forceinline__ void drop_add(const Drop& d, unsigned long long i, const Vec<T>& x, const Vec<T>& res, Vec<T>& out) {
+template <typename T, bool DROP, bool STRADDLE = false, bool WAVE = false>
+__device__ __forceinline__ void drop_add(const Drop& d, unsigned long long i, const Vec<T>& x, const Vec<T>& res, Vec<T>& out, bool edge = false, int left = 0) {
     constexpr int N = Vec<T>::N;
     unsigned w[N / 2];
-    if constexpr (DROP) drop_bits<N>(d, i, w);
+    if constexpr (DROP) drop_bits<N, STRADDLE, WAVE>(d, i, edge, left, w);
     float s[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -237,10 +249,11 @@ template <typename T, bool DROP> __device__ __forceinline__ void drop_add(const 
 }
 
 // out = kept ? v * scale : 0
-template <typename T> __device__ __forceinline__ void drop_only(const Drop& d, unsigned long long i, const float (&v)[Vec<T>::N], Vec<T>& out) {
+template <typename T, bool STRADDLE = false, bool WAVE = false>
+__device__ __forceinline__ void drop_only(const Drop& d, unsigned long long i, const float (&v)[Vec<T>::N], Vec<T>& out, bool edge = false, int left = 0) {
     constexpr int N = Vec<T>::N;
     unsigned w[N / 2];
-    drop_bits<N>(d, i, w);
+    drop_bits<N, STRADDLE, WAVE>(d, i, edge, left, w);
     float s[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = drop_kept<N>(d, w, j) ? v[j] * d.scale : 0.f;

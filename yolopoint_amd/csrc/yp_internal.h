@@ -112,15 +112,17 @@ __device__ __forceinline__ void yp_block_amax(float mx, float* amax) {
 
 // Philox4x32-10 (Salmon et al., SC 2011): the four words of the 128-bit counter (ctr, stream) under a 64-bit key.
 struct YpU4 { unsigned x, y, z, w; };
-__device__ __forceinline__ YpU4 yp_philox4x32(unsigned long long seed, unsigned long long ctr, unsigned long long stream) {
+// SCALAR: for a counter that is the same in the whole wave, in instructions that the scalar unit has.
+template <bool SCALAR = false> __device__ __forceinline__ YpU4 yp_philox4x32(unsigned long long seed, unsigned long long ctr, unsigned long long stream) {
     unsigned c0 = (unsigned)ctr, c1 = (unsigned)(ctr >> 32), c2 = (unsigned)stream, c3 = (unsigned)(stream >> 32);
     unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const unsigned hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
         const unsigned hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-        // (bitop3 0x96 = a ^ b ^ c in one instruction)
-        c0 = __builtin_amdgcn_bitop3_b32(hi1, c1, k0, 0x96); c1 = lo1; c2 = __builtin_amdgcn_bitop3_b32(hi0, c3, k1, 0x96); c3 = lo0;
+        if constexpr (SCALAR) { c0 = hi1 ^ c1 ^ k0; c2 = hi0 ^ c3 ^ k1; }
+        else { c0 = __builtin_amdgcn_bitop3_b32(hi1, c1, k0, 0x96); c2 = __builtin_amdgcn_bitop3_b32(hi0, c3, k1, 0x96); }     // (0x96: a ^ b ^ c in one instruction)
+        c1 = lo1; c3 = lo0;
         k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
     }
     return YpU4{c0, c1, c2, c3};
