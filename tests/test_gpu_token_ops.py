@@ -170,6 +170,20 @@ def test_layer_norm_hard_rows(cuda):
     assert bool(ops.layer_norm(torch.zeros(2, 5, device=cuda), eps=0.0).isnan().all())     # 0 / 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_norm_far_from_zero(cuda, dtype):
+    """Rows whose deviation is one step of their type: the rounding of the mean must not show.  (x - mean) is exact, the mean's rounding is taken off, so
+    y is off by a few 2^-24 of itself in fp32 and f16; bf16: by the mean's rounding, 4 * 2^-24 of 2^8 deviations."""
+    dt = TYPES[dtype]
+    step = torch.finfo(dt).eps * 1024.0
+    g = torch.Generator().manual_seed(1)
+    for D in (64, 777, 5000):
+        x = (1024.0 + step * torch.randint(0, 3, (9, D), generator=g).double()).to(dt)
+        y, _, rstd, xhat = O.layer_norm(x, None, None, 0.0 if dtype == "f32" else 1e-9)
+        got = ops.layer_norm(x.to(cuda), eps=0.0 if dtype == "f32" else 1e-9)
+        near(got, y, xhat.abs() + 1.0, 4 * 2.0 ** -24 * 1024.0 * float(rstd.max()) if dtype == "bf16" else 0.0)
+
+
 def test_layer_norm_large_strides(cuda):
     """Rows more than 2^31 elements into a tensor."""
     base = torch.zeros((1 << 31) + 4096, dtype=torch.bfloat16, device=cuda)
@@ -299,6 +313,20 @@ def test_fused_equals_its_parts_and_the_formula(cuda, D, dtype):
         with torch.no_grad():
             y2, z2 = ops.dropout_add_layer_norm(x, r, w, b, p=p, rng=rng)
         assert torch.equal(y, y2) and torch.equal(z, z2)
+
+
+def test_fused_of_a_tensor_with_itself_and_dropped_whole(cuda):
+    """x and residual the same leaf: its gradient is the sum of both.  p = 1: the residual's norm, no gradient through the branch."""
+    x, dy, dz = (make(cuda, (21, 88), torch.float32, i) for i in range(3))
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    for p in (0.0, 0.4):
+        one = torch.autograd.grad(ops.dropout_add_layer_norm(a, a, p=p, rng=(1, 2)), a, (dy, dz))[0]
+        two = torch.autograd.grad(ops.dropout_add_layer_norm(a, b, p=p, rng=(1, 2)), (a, b), (dy, dz))
+        assert torch.equal(one, two[0] + two[1])
+    y, z = ops.dropout_add_layer_norm(a, b, p=1.0, rng=(1, 2))
+    assert torch.equal(z, b) and torch.equal(y, ops.layer_norm(b))
+    da, db = torch.autograd.grad((y, z), (a, b), (dy, dz))
+    assert not da.any() and bool(db.any())
 
 
 def test_fused_many_rows(cuda):
@@ -497,6 +525,7 @@ def test_refusals(cuda):
              lambda: ops.layer_norm(x.half(), w.half(), w), lambda: ops.layer_norm(x, w.cpu()), lambda: ops.layer_norm(x, eps=-1.0), lambda: ops.layer_norm(x, eps=float("nan")),
              lambda: ops.layer_norm(torch.zeros((), device=cuda)), lambda: ops.layer_norm(x[:, :0]), lambda: ops.layer_norm(torch.zeros(1, 16385, device=cuda)),
              lambda: ops.dropout(x, 0.5, None), lambda: ops.dropout(x, -0.1, (1, 2)), lambda: ops.dropout(x, 1.1, (1, 2)), lambda: ops.dropout(x, float("nan"), (1, 2)),
+             lambda: ops.dropout(x, 0.5, 7), lambda: ops.dropout(x, 0.5, (1, 2, 3)), lambda: ops.dropout(x, 0.5, (1.5, 2)), lambda: ops.dropout(x, "a", (1, 2)),
              lambda: ops.dropout(x, 0.5, (1 << 64, 0)), lambda: ops.dropout(x, 0.5, (-1, 0)), lambda: ops.dropout(x, 0.5, torch.tensor([1, 2])),
              lambda: ops.dropout(x, 0.5, torch.tensor([1, 2], dtype=torch.int32, device=cuda)), lambda: ops.dropout(x, 0.5, torch.tensor([1, 2, 3], device=cuda)),
              lambda: ops.dropout(x, 0.5, (1, 2), residual=x[:2]), lambda: ops.dropout(x, 0.5, (1, 2), residual=x.half()), lambda: ops.dropout(x, 0.5, (1, 2), residual=x.cpu()),
@@ -587,6 +616,81 @@ def test_captured_training_pass_draws_new_masks(cuda):
     for (_, out, _), seed, base in zip(runs, (11, 12), (4, 44)):
         eager = step([t.clone().requires_grad_() for t in (data[0], data[1], w0, b0)], data[2], data[3], (seed, base))
         assert all(torch.equal(p, q) for p, q in zip(out, eager))
+
+
+def test_captured_first_call_of_a_wide_norm(cuda):
+    """The largest rows, forward and backward captured with no call before: what the launches ask the runtime for may be asked during a capture."""
+    D = 16000
+    x0, dy, w0 = make(cuda, (7, D), torch.float16, 1), make(cuda, (7, D), torch.float16, 2), make(cuda, (D,), torch.float16, 3)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        x, w = x0.clone().requires_grad_(), w0.clone().requires_grad_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        y = ops.layer_norm(x, w)
+        out = (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        ex, ew = x.detach().clone().requires_grad_(), w0.clone().requires_grad_()
+        ey = ops.layer_norm(ex, ew)
+        assert all(torch.equal(p, q) for p, q in zip(out, (ey, *torch.autograd.grad(ey, (ex, ew), dy)))), i
+        with torch.no_grad():
+            x.mul_(0.5)
+
+
+def test_calls_from_two_threads(cuda):
+    """Two threads on two streams, forward and backward: each gets its own results."""
+    import threading
+    data = [[make(cuda, (600 + 40 * i, 96 + 32 * i), torch.bfloat16, 4 * i + j) for j in range(3)] for i in range(2)]
+
+    def work(x, r, dy, seed):
+        x, r = x.clone().requires_grad_(), r.clone().requires_grad_()
+        y, z = ops.dropout_add_layer_norm(x, r, p=0.3, rng=(seed, 1))
+        return (y.detach(), z.detach(), *torch.autograd.grad((y, z), (x, r), (dy, dy)))
+    want = [work(*d, i) for i, d in enumerate(data)]
+    torch.cuda.synchronize()
+    got, bad = [None, None], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got[i] = work(*data[i], i)
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+        except BaseException as e:                                                   # noqa: BLE001
+            bad.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
+def test_saved_tensors_go_through_hooks(cuda):
+    """What the backward pass reads passes the saved-tensor hooks (offloading): gradients are the same."""
+    x, w, dy = make(cuda, (33, 64), torch.bfloat16, 1).requires_grad_(), make(cuda, (64,), torch.float32, 2).requires_grad_(), make(cuda, (33, 64), torch.bfloat16, 3)
+    want = torch.autograd.grad(ops.layer_norm(x, w), (x, w), dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(cuda)):
+        y = ops.layer_norm(x, w)
+    got = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_shared_heads_sum_their_gradients(cuda):
+    """One key head expanded over the query heads: autograd sums what the expanded view gets."""
+    B, T, H, D = 2, 9, 4, 32
+    inv = ops.rotary_frequencies(D)[0].to(cuda)
+    k, dk = make(cuda, (B, T, 1, D), torch.float32, 1).requires_grad_(), make(cuda, (B, T, H, D), torch.float32, 2)
+    got, = torch.autograd.grad(ops.rotary(k.expand(B, T, H, D), 5, inv), k, dk)
+    each = ops.rotary(k.detach(), 5, inv)
+    assert torch.equal(ops.rotary(k.expand(B, T, H, D), 5, inv), each.expand(B, T, H, D))
+    want = O.rotary(dk.cpu(), torch.arange(T) + 5, inv.cpu(), False, "bthd", 1.0, True).sum(2, keepdim=True)
+    near(got, want, dk.cpu().double().abs().sum((2, 3), keepdim=True))
 
 
 def test_captured_serving_step(cuda):

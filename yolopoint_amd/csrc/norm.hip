@@ -18,13 +18,15 @@ struct LnFwd {
     float scale;
 };
 
-// mean = sum x / D;  var = sum (x - mean)^2 / D;  y = (x - mean) / sqrt(var + eps) w + b.  fp32 rows: delta = sum (x - mean) / D is what rounding left
-// of the mean, and is taken off as well (a row of mean 4096 and deviation 1 keeps 1e-7 instead of 1e-3; 16-bit rows have no such digits).
+// mean = sum x / D;  var = sum (x - mean)^2 / D;  y = (x - mean) / sqrt(var + eps) w + b.  Behind the mean, delta = sum (x - mean) / D is what rounding
+// left of it, and is taken off as well: a fp32 row of mean 4096 and deviation 1 keeps 1e-7 instead of 1e-3, a f16 row of mean 1000 and deviation 1/4
+// (one step of its type) 1e-7 instead of its half step.  bf16 rows have no such digits (a deviation of one step is 2^-8 of the mean, the mean's
+// rounding 2^-24 of it), and do without the second sum (two of some twenty instructions a value).
 // The next row is on its way while this one is worked on (the first before the weights are read).
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
     constexpr int N = Vec<T>::N, NC = E / N, ROWS = G ? 256 / G : 1;
-    constexpr bool FINE = sizeof(T) == 4;
+    constexpr bool FINE = !__is_same(T, __bf16);
     __shared__ float2 sh[2][16];
     const T *x = (const T*)a.x, *res = (const T*)a.res;
     T *z = (T*)a.z, *y = (T*)a.y;

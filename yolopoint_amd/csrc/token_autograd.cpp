@@ -512,9 +512,9 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
         if (q.stride(3) != 1 || (k && k->stride(3) != 1)) fail("rotary: dense features in place");
         if (q.numel() + (k ? k->numel() : 0) == 0) return {q, k};
         if (!apart(q) || (k && (!apart(*k) || !separate(q, *k, heads_first)))) fail("rotary: q and k hold each element once in place");
-        turn_launch(q, k_, q, k_, positions_, inv_freq, how, false);
-        q.unsafeGetTensorImpl()->bump_version();
+        q.unsafeGetTensorImpl()->bump_version();            // (refuses an inference tensor outside inference mode)
         if (k) k_.unsafeGetTensorImpl()->bump_version();
+        turn_launch(q, k_, q, k_, positions_, inv_freq, how, false);
         return {q, k};
     }
     std::pair<Tensor, Tensor> out;

@@ -48,7 +48,12 @@ def _state(what, p, rng):
         if p != 0.0:
             raise _hip.YpError(f"{what}: p > 0 needs rng = (seed, offset)")
         return 0, 0, None
-    seed, offset = rng
+    try:
+        seed, offset = rng
+    except TypeError:
+        raise _hip.YpError(f"{what}: rng = (seed, offset), not {type(rng).__name__}") from None
+    except ValueError:
+        raise _hip.YpError(f"{what}: rng is two numbers") from None
     return seed, offset, None
 
 
