@@ -5,6 +5,8 @@
 
 namespace {
 
+// Bound by HBM: 67.1 M bf16 elements take 40.6 us (6.6 TB/s), with a residual 72.4 us (5.6 TB/s; a large copy 5.2 - 5.4).  Eight bf16 elements a thread are
+// one call of the generator (some 85 instructions), four fp32 ones use half of theirs, for the same 16 bytes: 40.2 us for the same 256 MB.
 template <typename T, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y, int64_t n, unsigned long long seed,
                                                       unsigned long long offset, const int64_t* __restrict__ rng, unsigned threshold, float scale) {
@@ -59,6 +61,9 @@ __device__ __forceinline__ void turn_cos_sin(double turns, float& c, float& s) {
     s = (iq & 2) ? -b : b;
 }
 
+// Bound by HBM from two heads a thread on: 4 x 8192 tokens of 20 x 128 bf16 (335 MB moved) take 65 us, 5.2 TB/s, as a large copy.  A single head of bf16
+// is bound by its cosines instead (some 40 instructions a pair, half of them 64-bit: 3.8 TB/s).  The angles are formed here and not read from a table of
+// cosines: such a table is another 2 x 4 bytes a pair and token, as much as one bf16 head moves, and ends at the longest context it was made for.
 // A thread owns one chunk of a head's pairs (16 bytes of each half, or 32 bytes of interleaved pairs) of one token, and walks the heads slot, slot + hs,
 // ... of q and then of k with the same cosines and sines.
 template <typename T, Tail TAIL>
@@ -181,8 +186,9 @@ extern "C" int yp_rotary(const YpRotaryDesc* d, void* stream) {
     a.scale = d->scale; a.sign = d->inverse ? -1.f : 1.f; a.interleaved = d->interleaved != 0; a.in_place = d->q == d->q_out && d->k == d->k_out;
     const int N = d->dtype == YP_F32 ? 4 : 8, H = d->Hq + d->Hk;
     const int chunks = (d->R / 2 + N - 1) / N + (a.in_place ? 0 : (d->D - d->R + 2 * N - 1) / (2 * N));
-    // heads beside each other: all of them while the tokens alone do not fill the chip, else four to a thread (they share its cosines)
-    const bool few = (int64_t)a.tokens * H * chunks <= 256 * 2048;
+    // heads beside each other: all of them while even that does not fill the chip (64 tokens of 20 x 128 bf16: 3.8 us against 5.2 with four to a thread),
+    // else four to a thread, which share its cosines (4096 tokens: 10.8 us against 17.6; the two meet at some 150 thousand threads)
+    const bool few = (int64_t)a.tokens * H * chunks <= 256 * 512;
     int hs = few ? H : (H + 3) / 4;
     if (hs > 256 / chunks) hs = 256 / chunks;
     a.hs = hs;
