@@ -562,6 +562,79 @@ def test_written_inputs_are_refused_in_the_backward_pass(cuda):
         y.sum().backward()
 
 
+def test_frequencies_are_a_table(cuda):
+    """A table that asks for a gradient would get none: refused."""
+    q = torch.randn(2, 5, 3, 8, device=cuda)
+    inv = ops.rotary_frequencies(8)[0].to(cuda).requires_grad_()
+    for kw in ({}, {"inplace": True}):
+        with pytest.raises(_hip.YpError, match="no gradient"):
+            ops.rotary(q, 0, inv, **kw)
+
+
+def test_a_written_state_is_refused_in_the_backward_pass(cuda):
+    x = torch.randn(4, 8, device=cuda, requires_grad=True)
+    for f in (lambda s: ops.dropout(x, 0.5, s), lambda s: ops.dropout_add_layer_norm(x, x, p=0.5, rng=s)[0]):
+        state = torch.tensor([3, 4], device=cuda)
+        y = f(state)
+        state[1] += 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_a_graph_kept_for_a_second_pass(cuda):
+    """retain_graph: the second pass gives the same bits; without it, what was saved is gone."""
+    x, w = make(cuda, (37, 100), torch.bfloat16, 1).requires_grad_(), make(cuda, (100,), torch.float32, 2).requires_grad_()
+    inv = ops.rotary_frequencies(20)[0].to(cuda)
+    at = torch.arange(37, device=cuda)
+    y = ops.rotary(ops.dropout_add_layer_norm(ops.layer_norm(x, w), ops.dropout(x, 0.2, (5, 6)), w, p=0.1, rng=(5, 7))[0].view(1, 37, 5, 20), at, inv)
+    dy = make(cuda, (1, 37, 5, 20), torch.bfloat16, 3)
+    first = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    second = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, (x, w), dy)
+
+
+def test_inference_mode(cuda):
+    """Inference tensors: results as under no_grad; in place too."""
+    x, w = make(cuda, (9, 64), torch.float16, 1), make(cuda, (64,), torch.float16, 2).requires_grad_()
+    inv = ops.rotary_frequencies(32)[0].to(cuda)
+    with torch.no_grad():
+        want = ops.dropout_add_layer_norm(x, x, w, p=0.3, rng=(1, 2)), ops.rotary(x.view(1, 9, 2, 32), 7, inv)
+    with torch.inference_mode():
+        got = ops.dropout_add_layer_norm(x, x, w, p=0.3, rng=(1, 2)), ops.rotary(x.view(1, 9, 2, 32), 7, inv)
+        q = x.clone().view(1, 9, 2, 32)
+        ops.rotary(q, 7, inv, inplace=True)
+        assert torch.equal(q, want[1])
+        assert torch.equal(ops.layer_norm(got[0][1], w), want[0][0])
+    assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[0][1], want[0][1]) and torch.equal(got[1], want[1])
+
+
+def test_views_that_are_negated_when_read(cuda):
+    """The imaginary part of a conjugate holds its values with the other sign: operands, positions and gradients."""
+    c = torch.complex(make(cuda, (50, 1), torch.float32, 1), make(cuda, (50, 1), torch.float32, 2)).conj()
+    x, r = c.imag, make(cuda, (50, 1), torch.float32, 3)
+    assert x.is_neg()
+    dense = x.clone()
+    assert not dense.is_neg()
+    assert torch.equal(ops.dropout_add_layer_norm(x, r)[1], dense + r) and torch.equal(ops.dropout_add_layer_norm(r, x)[1], dense + r)
+    assert torch.equal(ops.dropout(x, 0.5, (1, 2), residual=x), ops.dropout(dense, 0.5, (1, 2), residual=dense))
+    w = c[:1, 0].imag
+    assert torch.equal(ops.layer_norm(r, None, w), ops.layer_norm(r, None, w.clone()))
+    inv = ops.rotary_frequencies(8)[0].to(cuda)
+    q = make(cuda, (1, 50, 3, 8), torch.float32, 4)
+    assert torch.equal(ops.rotary(q, x[:, 0], inv), ops.rotary(q, dense[:, 0].contiguous(), inv))
+    a = r.clone().requires_grad_()
+    got, = torch.autograd.grad(ops.dropout_add_layer_norm(a, r, p=0.5, rng=(1, 2)), a, (x, x))
+    want, = torch.autograd.grad(ops.dropout_add_layer_norm(a, r, p=0.5, rng=(1, 2)), a, (dense, dense))
+    assert torch.equal(got, want)
+    view = torch._neg_view(q)
+    got = ops.rotary(view, 3, inv)
+    assert torch.equal(got, ops.rotary(-q, 3, inv))
+    with pytest.raises(_hip.YpError):
+        ops.rotary(view, 3, inv, inplace=True)
+
+
 # ------------------------------------------------------------------------------------------------------------------ streams and graphs
 def test_side_stream(cuda):
     """Launches go to the current stream: work queued in front of them on it is seen without a synchronisation."""

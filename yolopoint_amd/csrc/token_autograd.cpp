@@ -84,9 +84,13 @@ variable_list once(variable_list&& grads) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- rows
+// t as it lies if it is dense, else a dense copy (also of a view that is negated when it is read, as the imaginary part of a conjugate is)
+Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+
 // x with rows of one distance where they lie, anything else through a dense copy
 struct Rows { Tensor t; int64_t stride; };
-Rows rows_of(const Tensor& x) {
+Rows rows_of(const Tensor& t) {
+    const Tensor x = t.resolve_neg();
     const int64_t D = x.size(-1);
     if (x.is_contiguous()) return {x, D};
     if (D == 1 || x.stride(-1) == 1) {
@@ -121,7 +125,7 @@ void check_norm(const char* what, const Tensor& x, const MaybeTensor& w, const M
 
 void check_drop(const char* what, const Tensor& x, double p, const MaybeTensor& rng) {
     if (!(p >= 0.0 && p <= 1.0)) fail("%s: a rate of 0 to 1, not %g", what, p);
-    if (rng && (rng->scalar_type() != at::kLong || rng->dim() != 1 || rng->size(0) != 2 || !rng->is_contiguous() || rng->device() != x.device()))
+    if (rng && (rng->scalar_type() != at::kLong || rng->dim() != 1 || rng->size(0) != 2 || !rng->is_contiguous() || rng->is_neg() || rng->device() != x.device()))
         fail("%s: rng as a tensor is int64 [seed, offset] on %s", what, x.device().str().c_str());
 }
 
@@ -132,7 +136,7 @@ struct NormResult { Tensor y, z, stats; };                 // stats: fp32 [2, ro
 NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias, double eps, const Dropping& drop, const Tensor& rng, bool keep) {
     const int64_t D = x.size(-1), rows = x.numel() / D;
     const Rows xr = rows_of(x);
-    const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+    const Tensor w = dense(weight), b = dense(bias);
     NormResult r;
     r.y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
     YpLayerNormDesc d{};
@@ -175,6 +179,7 @@ struct NormBackward : Node {
 
     std::string name() const override { return fused ? "DropoutAddLayerNormBackward" : "LayerNormBackward"; }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         z.reset_data();
         weight.reset_data();
         stats.reset_data();
@@ -182,6 +187,7 @@ struct NormBackward : Node {
     }
     // gradients of (x, weight, bias), or of (x, residual, weight, bias)
     variable_list apply(variable_list&& in) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         const int n = fused ? 4 : 3;
         variable_list out(n);
         Tensor dy = in[0], dz = fused ? in[1] : Tensor();
@@ -194,7 +200,7 @@ struct NormBackward : Node {
             const int64_t D = z_.size(-1), rows = z_.numel() / D;
             const Rows zr = rows_of(z_), dyr = rows_of(dy);
             Rows dzr;
-            const Tensor w = w_.defined() ? w_.contiguous() : w_;
+            const Tensor w = dense(w_);
             const auto options = z_.options().memory_format(at::MemoryFormat::Contiguous);
             const Tensor dres = at::empty(z_.sizes(), options);
             const bool drops = drop.p * 65536.0 + 0.5 >= 1.0;
@@ -295,7 +301,7 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const MaybeTe
 
 // ---------------------------------------------------------------------------------------------------------------- dropout
 Tensor drop_launch(const Tensor& x, const Tensor& residual, const Dropping& drop, const Tensor& rng) {
-    const Tensor xc = x.contiguous(), rc = residual.defined() ? residual.contiguous() : residual;
+    const Tensor xc = dense(x), rc = dense(residual);
     Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
     check(lib.dropout(xc.data_ptr(), address(rc), y.data_ptr(), x.numel(), type_code(x.scalar_type()), drop.p, drop.seed, drop.offset, (const int64_t*)address(rng), stream_of(x)));
     return y;
@@ -306,8 +312,12 @@ struct DropoutBackward : Node {
     Dropping drop;
 
     std::string name() const override { return "DropoutBackward"; }
-    void release_variables() override { rng.reset_data(); }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        rng.reset_data();
+    }
     variable_list apply(variable_list&& in) override {     // gradients of (x, residual)
+        std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(2);
         const Tensor dy = in[0];
         if (!dy.defined()) return out;
@@ -400,7 +410,7 @@ void turn_launch(const Tensor& q, const Tensor& k, const Tensor& q_out, const Te
     check(lib.rotary(&d, stream_of(q)));
 }
 
-Tensor feature_dense(const Tensor& x) { return !x.defined() || x.stride(3) == 1 ? x : x.contiguous(); }
+Tensor feature_dense(const Tensor& x) { return x.defined() && x.stride(3) == 1 && !x.is_neg() ? x : dense(x); }
 
 std::pair<Tensor, Tensor> turned(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, const Turn& how, bool inverse) {
     const Tensor qd = feature_dense(q), kd = feature_dense(k);
@@ -417,10 +427,12 @@ struct RotaryBackward : Node {
 
     std::string name() const override { return "RotaryBackward"; }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         positions.reset_data();
         inv_freq.reset_data();
     }
     variable_list apply(variable_list&& in) override {     // gradients of (q, k)
+        std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(2);
         const Tensor dq = task_should_compute_output(0) ? in[0] : Tensor(), dk = has_k && task_should_compute_output(1) ? in[1] : Tensor();
         const Tensor first = dq.defined() ? dq : dk, second = dq.defined() ? dk : Tensor();
@@ -482,6 +494,7 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
     if (q.dim() != 4 || q.size(3) < 2 || q.size(3) > 1024) fail("rotary: q of four dimensions, heads of 2 to 1024 features, not %s", shape_of(q).c_str());
     if (inv_freq.scalar_type() != at::kDouble || inv_freq.dim() != 1 || !inv_freq.is_contiguous() || inv_freq.numel() < 1 || 2 * inv_freq.numel() > q.size(3))
         fail("rotary: inv_freq is float64 [R / 2] with R <= the head's features");
+    if (inv_freq.requires_grad() || inv_freq.is_neg()) fail("rotary: inv_freq is a plain table and has no gradient");
     const int64_t B = batch_of(q), T = tokens_of(q, heads_first);
     const int64_t most = (int64_t)1 << 31;
     if (B >= most || T >= most || (T && B >= (most + T - 1) / T) || heads_of(q, heads_first) >= most / 2) fail("rotary: fewer than 2^31 tokens a call");
@@ -505,11 +518,11 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
         }
     }
     const c10::DeviceGuard guard(q.device());
-    const Tensor k_ = given(k), positions_ = given(positions);
+    const Tensor k_ = given(k), positions_ = positions ? positions->resolve_neg() : Tensor();
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || wants(k));
     if (inplace) {
         if (grad) fail("rotary: no gradients in place");
-        if (q.stride(3) != 1 || (k && k->stride(3) != 1)) fail("rotary: dense features in place");
+        if (q.stride(3) != 1 || q.is_neg() || (k && (k->stride(3) != 1 || k->is_neg()))) fail("rotary: dense features in place");
         if (q.numel() + (k ? k->numel() : 0) == 0) return {q, k};
         if (!apart(q) || (k && (!apart(*k) || !separate(q, *k, heads_first)))) fail("rotary: q and k hold each element once in place");
         q.unsafeGetTensorImpl()->bump_version();            // (refuses an inference tensor outside inference mode)

@@ -15,6 +15,7 @@ import importlib.util
 import ctypes as C
 import math
 import os
+import threading
 
 import torch
 
@@ -23,20 +24,27 @@ from .. import _hip
 _PATH = os.path.join(os.path.dirname(_hip.LIB_PATH), "_token_autograd.so")
 _ENTRIES = ("yp_last_error", "yp_layer_norm_fwd", "yp_layer_norm_bwd", "yp_layer_norm_bwd_workspace_bytes", "yp_layer_norm_max_width", "yp_dropout", "yp_rotary")
 _module = None
+_lock = threading.Lock()
+
+
+def _load():
+    lib = _hip.lib()
+    if not os.path.exists(_PATH):
+        raise _hip.YpError(f"{_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    loader = importlib.machinery.ExtensionFileLoader("_token_autograd", _PATH)
+    m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_token_autograd", loader))
+    loader.exec_module(m)
+    m.init([C.cast(getattr(lib, n), C.c_void_p).value for n in _ENTRIES], _hip.YpError)
+    return m
 
 
 def _native():
     """The C++ side (csrc/token_autograd.cpp: checks, buffers, launches, autograd nodes), over the entry points of the library that is loaded."""
     global _module
     if _module is None:
-        lib = _hip.lib()
-        if not os.path.exists(_PATH):
-            raise _hip.YpError(f"{_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
-        loader = importlib.machinery.ExtensionFileLoader("_token_autograd", _PATH)
-        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_token_autograd", loader))
-        loader.exec_module(m)
-        m.init([C.cast(getattr(lib, n), C.c_void_p).value for n in _ENTRIES], _hip.YpError)
-        _module = m
+        with _lock:
+            if _module is None:
+                _module = _load()
     return _module
 
 
@@ -137,7 +145,7 @@ def rotary(q, positions, inv_freq, k=None, interleaved=False, layout="bthd", sca
     their head numbers may differ.  Pairs: (j, j + R / 2), or (2 j, 2 j + 1) when interleaved, R = 2 * len(inv_freq) <= D <= 1024; the rest of a head is copied.
     positions: an int (token t stands at positions + t), or a tensor of int32, int64 or float32: [T], [1, T] or [B, T]; with a last dimension of 2
     ([T, 2], [B, T, 2], keypoints at (x, y)) the first half of the pairs turns by the first, the second half by the second.  A [B, 2] tensor is [B, T = 2].
-    inv_freq, scale: from `rotary_frequencies`; the table is float64 on the tensors' device, angles are formed in 64 bits (positions of 10^6 keep 1e-7 of a turn).
+    inv_freq, scale: from `rotary_frequencies`; the table is float64 on the tensors' device and has no gradient, angles are formed in 64 bits (positions of 10^6 keep 1e-7 of a turn).
     inplace: write into q and k (no gradients; refused where an element would be turned twice: expanded tensors, q and k that meet).  Gradients: q, k
     (turned back)."""
     if layout not in ("bthd", "bhtd"):
