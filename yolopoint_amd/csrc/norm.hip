@@ -24,8 +24,8 @@ struct LnFwd {
 // rounding 2^-24 of it), and do without the second sum (two of some twenty instructions a value).
 // The next row is on its way while this one is worked on (the first before the weights are read): its registers are not touched before its turn, or the
 // wait for them would stand right behind the loads.
-// Measured, 128 MiB a tensor: 44 - 60 us for widths 16 .. 16384 (4.5 - 6.2 TB/s), with residual and dropout 99 - 125 us (4.3 - 5.4; a large copy: 5.2 - 5.4);
-// bf16 widths just over a border with dropout are bound by their instructions (4100: 141 us).
+// Measured, 128 MiB a tensor: 44 - 60 us for widths 16 .. 16384 (4.5 - 6.2 TB/s), with residual and dropout 100 - 130 us (4.1 - 5.4; a large copy: 5.2 - 5.4);
+// widths just over a border with dropout are bound by their instructions (bf16 4100: 142 us, 4099: 158).
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
     constexpr int N = Vec<T>::N, NC = E / N, ROWS = G ? 256 / G : 1;

@@ -25,7 +25,7 @@ struct LnBwd {
 // 16-byte pieces: no bank twice); between the sums and the result the row waits in the type it was loaded in, and xhat and h are formed again (the
 // empty asm keeps the compiler from holding them in fp32 instead); one chunk after the other, so that only one's random numbers are live.
 // Measured, 128 MiB a tensor: 80 - 104 us for widths 16 .. 16384 (3.9 - 5.1 TB/s over the two tensors read and one written), through residual and dropout
-// 129 - 154 us (4.4 - 5.2 over five); odd bf16 widths with dropout are bound by their instructions (2100: 231 us), fp32 rows of more than 8192 features by
+// 130 - 156 us (4.3 - 5.1 over five); odd bf16 widths with dropout are bound by their instructions (777: 168, 2100: 210, 4099: 236 us), fp32 rows of more than 8192 features by
 // registers that do not suffice (16384: 204 us).
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a) {
@@ -246,7 +246,7 @@ LnShape ln_shape(int D) {
 
 // Workgroups: what the chip holds beside each other, 24 waves a compute unit at the most (each writes a line of partial sums, so there are no more of them).
 // `fit`: workgroups that a compute unit holds, by the kernel's registers; unknown (the workspace's size): 24 waves.  A grid that a part of the
-// compute units hold twice and the others once leaves those idle for half of the time: 80 against 92 us for 262144 x 256 fp32.
+// compute units hold twice and the others once leaves those idle for half of the time: 84 against 90 us for 87381 x 384 fp32.
 int ln_bwd_blocks(int64_t rows, int D, int fit) {
     const LnShape s = ln_shape(D);
     const int cap = 24 * 64 / s.block > 1 ? 24 * 64 / s.block : 1, per_cu = fit > 0 && fit < cap ? fit : cap;

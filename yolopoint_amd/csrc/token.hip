@@ -5,8 +5,8 @@
 
 namespace {
 
-// Bound by HBM: 67.1 M bf16 elements take 40.6 us (6.6 TB/s), with a residual 72.4 us (5.6 TB/s; a large copy 5.2 - 5.4).  Eight bf16 elements a thread are
-// one call of the generator (some 85 instructions), four fp32 ones use half of theirs, for the same 16 bytes: 40.2 us for the same 256 MB.
+// Bound by HBM: 67.1 M bf16 elements take 42 us (6.4 TB/s), with a residual 74 us (5.5 TB/s; a large copy 5.2 - 5.4).  Eight bf16 elements a thread are
+// one call of the generator (some 85 instructions), four fp32 ones use half of theirs, for the same 16 bytes: 40.4 us for the same 256 MB.
 template <typename T, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y, int64_t n, unsigned long long seed,
                                                       unsigned long long offset, const int64_t* __restrict__ rng, unsigned threshold, float scale) {

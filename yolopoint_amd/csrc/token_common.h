@@ -9,11 +9,6 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
-template <int DT> struct Sc;
-template <> struct Sc<YP_F16> { using t = _Float16; };
-template <> struct Sc<YP_BF16> { using t = __bf16; };
-template <> struct Sc<YP_F32> { using t = float; };
-
 // ------------------------------------------------------------------------------------------------------------------ memory
 // 16 bytes of a row.  Rows may start on any element (odd widths, slices of wider rows): the target's global loads and stores take any alignment,
 // so there is no separate path for unaligned rows.
@@ -177,8 +172,8 @@ template <int G> __device__ __forceinline__ float lanes_sum(float v) {
 
 // ------------------------------------------------------------------------------------------------------------------ dropout
 // Element i of a tensor (flat, row-major) is kept where half i % 8 of the 128 bits that Philox4x32-10 gives for the counter (i / 8, offset) is
-// >= threshold = round(65536 p).  16 bits an element: the rate moves in steps of 2^-16, and one call of the generator (20 multiplications of
-// quarter rate) serves eight elements.
+// >= threshold = round(65536 p).  16 bits an element: the rate moves in steps of 2^-16, and one call of the generator (some 85
+// instructions) serves eight elements.
 struct Drop {
     unsigned long long seed, offset;
     unsigned threshold;
@@ -194,9 +189,9 @@ __device__ __forceinline__ Drop drop_state(unsigned long long seed, unsigned lon
 // words too (rows of odd widths).  Those are what the next lane has just made of the counter after this one, so they come from there; `edge`: this
 // lane is the last of its row's lanes in the wave; `left`: elements of the row from i on.  A wave that holds one row (WAVE) makes the words of its last
 // lane's next counter on the scalar unit, beside the other waves' vector work.
-template <int N, bool STRADDLE, bool WAVE> __device__ __forceinline__ void drop_bits(const Drop& d, unsigned long long i, bool edge, int left, unsigned (&w)[N / 2]) {
+template <int N, bool STRADDLE, bool WAVE, bool MAD> __device__ __forceinline__ void drop_bits(const Drop& d, unsigned long long i, bool edge, int left, unsigned (&w)[N / 2]) {
     const unsigned sh = WAVE && N == 8 ? __builtin_amdgcn_readfirstlane((unsigned)i & 7u) : (unsigned)i & 7u;       // (chunks of 8: the same for a row)
-    const YpU4 a = yp_philox4x32(d.seed, i >> 3, d.offset);
+    const YpU4 a = yp_philox4x32<false, MAD>(d.seed, i >> 3, d.offset);
     if constexpr (!STRADDLE) {                      // i % N == 0
         if constexpr (N == 8) { w[0] = a.x; w[1] = a.y; w[N / 2 - 2] = a.z; w[N / 2 - 1] = a.w; }
         else { w[0] = sh ? a.z : a.x; w[1] = sh ? a.w : a.y; }
@@ -207,9 +202,9 @@ template <int N, bool STRADDLE, bool WAVE> __device__ __forceinline__ void drop_
             YpU4 s;
             if constexpr (WAVE) {
                 const unsigned lo = __builtin_amdgcn_readlane((unsigned)(i >> 3), 63), hi = __builtin_amdgcn_readlane((unsigned)(i >> 35), 63);
-                s = yp_philox4x32<true>(d.seed, (((unsigned long long)hi << 32) | lo) + 1, d.offset);
+                s = yp_philox4x32<true, MAD>(d.seed, (((unsigned long long)hi << 32) | lo) + 1, d.offset);
             } else {
-                s = yp_philox4x32(d.seed, (i >> 3) + 1, d.offset);
+                s = yp_philox4x32<false, MAD>(d.seed, (i >> 3) + 1, d.offset);
             }
             b.x = edge ? s.x : b.x; b.y = edge ? s.y : b.y; b.z = edge ? s.z : b.z; b.w = edge ? s.w : b.w;
         }
@@ -237,7 +232,7 @@ template <typename T, bool DROP, bool STRADDLE = false, bool WAVE = false>
 __device__ __forceinline__ void drop_add(const Drop& d, unsigned long long i, const Vec<T>& x, const Vec<T>& res, Vec<T>& out, bool edge = false, int left = 0) {
     constexpr int N = Vec<T>::N;
     unsigned w[N / 2];
-    if constexpr (DROP) drop_bits<N, STRADDLE, WAVE>(d, i, edge, left, w);
+    if constexpr (DROP) drop_bits<N, STRADDLE, WAVE, false>(d, i, edge, left, w);
     float s[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -248,12 +243,15 @@ __device__ __forceinline__ void drop_add(const Drop& d, unsigned long long i, co
     out = to_vec<T>(s);
 }
 
-// out = kept ? v * scale : 0
+// out = kept ? v * scale : 0.  The generator's products as 64-bit multiply-adds for eight 16-bit elements, which its instructions bound (backward of
+// 31956 x 2100 bf16 210 us against 232, 86369 x 777 168 against 178, 13421 x 5000 132 against 149; at worst 16372 x 4099 236 against 231; dropout of
+// 8.4 M elements 8.4 against 8.9); as halves for four fp32 elements, where the pairs of registers cost more (8186 x 4099: 148 against 157) than the
+// products, and in drop_add (forward of 16372 x 4099 bf16: 159 against 187).
 template <typename T, bool STRADDLE = false, bool WAVE = false>
 __device__ __forceinline__ void drop_only(const Drop& d, unsigned long long i, const float (&v)[Vec<T>::N], Vec<T>& out, bool edge = false, int left = 0) {
     constexpr int N = Vec<T>::N;
     unsigned w[N / 2];
-    drop_bits<N, STRADDLE, WAVE>(d, i, edge, left, w);
+    drop_bits<N, STRADDLE, WAVE, N == 8>(d, i, edge, left, w);
     float s[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = drop_kept<N>(d, w, j) ? v[j] * d.scale : 0.f;

@@ -112,14 +112,20 @@ __device__ __forceinline__ void yp_block_amax(float mx, float* amax) {
 
 // Philox4x32-10 (Salmon et al., SC 2011): the four words of the 128-bit counter (ctr, stream) under a 64-bit key.
 struct YpU4 { unsigned x, y, z, w; };
-// SCALAR: for a counter that is the same in the whole wave, in instructions that the scalar unit has.
-template <bool SCALAR = false> __device__ __forceinline__ YpU4 yp_philox4x32(unsigned long long seed, unsigned long long ctr, unsigned long long stream) {
+// SCALAR: for a counter that is the same in the whole wave, in instructions that the scalar unit has.  MAD: each product as one 64-bit multiply-add
+// (one instruction and a pair of registers), not as its two halves.
+template <bool SCALAR = false, bool MAD = false> __device__ __forceinline__ YpU4 yp_philox4x32(unsigned long long seed, unsigned long long ctr, unsigned long long stream) {
     unsigned c0 = (unsigned)ctr, c1 = (unsigned)(ctr >> 32), c2 = (unsigned)stream, c3 = (unsigned)(stream >> 32);
     unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
-        const unsigned hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
-        const unsigned hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
+        unsigned hi0, lo0, hi1, lo1;
+        if constexpr (MAD) {
+            const unsigned long long p0 = 0xD2511F53ull * c0, p1 = 0xCD9E8D57ull * c2;
+            hi0 = (unsigned)(p0 >> 32); lo0 = (unsigned)p0; hi1 = (unsigned)(p1 >> 32); lo1 = (unsigned)p1;
+        } else {
+            hi0 = __umulhi(0xD2511F53u, c0); lo0 = 0xD2511F53u * c0; hi1 = __umulhi(0xCD9E8D57u, c2); lo1 = 0xCD9E8D57u * c2;
+        }
         if constexpr (SCALAR) { c0 = hi1 ^ c1 ^ k0; c2 = hi0 ^ c3 ^ k1; }
         else { c0 = __builtin_amdgcn_bitop3_b32(hi1, c1, k0, 0x96); c2 = __builtin_amdgcn_bitop3_b32(hi0, c3, k1, 0x96); }     // (0x96: a ^ b ^ c in one instruction)
         c1 = lo1; c3 = lo0;

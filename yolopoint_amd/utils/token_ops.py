@@ -1,7 +1,8 @@
 """Operators on tokens -- rows of features: keypoint descriptors, cells of the descriptor map, entries of a sequence -- for the transformer blocks
 that refine or match what the network extracts: layer norm (forward and backward), dropout + residual + layer norm in one pass, dropout from a
-counter-based generator whose mask is never stored, rotary positions (sequences, or keypoints at (x, y)).  Kernels: csrc/token.hip.  No
-reference counterpart: the reference's network is convolutional and its matcher is the mutual nearest neighbour (models/model_wrap.py:434-476).
+counter-based generator whose mask is never stored, rotary positions (sequences, or keypoints at (x, y)).  Kernels: csrc/token.hip,
+csrc/norm.hip, csrc/norm_bwd.hip.  No reference counterpart: the reference's network is convolutional and its matcher is the mutual nearest
+neighbour (models/model_wrap.py:434-476).
 
 All of them: float16, bfloat16 or float32 tensors on the GPU, any leading dimensions, rows that may start on any element (slices of wider tensors are read
 in place where their rows have one distance, else copied first); sums, statistics and angles in 32 bits or more, results rounded once;
@@ -145,7 +146,8 @@ def rotary(q, positions, inv_freq, k=None, interleaved=False, layout="bthd", sca
     their head numbers may differ.  Pairs: (j, j + R / 2), or (2 j, 2 j + 1) when interleaved, R = 2 * len(inv_freq) <= D <= 1024; the rest of a head is copied.
     positions: an int (token t stands at positions + t), or a tensor of int32, int64 or float32: [T], [1, T] or [B, T]; with a last dimension of 2
     ([T, 2], [B, T, 2], keypoints at (x, y)) the first half of the pairs turns by the first, the second half by the second.  A [B, 2] tensor is [B, T = 2].
-    inv_freq, scale: from `rotary_frequencies`; the table is float64 on the tensors' device and has no gradient, angles are formed in 64 bits (positions of 10^6 keep 1e-7 of a turn).
+    inv_freq, scale: from `rotary_frequencies`; the table is float64 on the tensors' device and has no gradient, angles are formed in 64 bits (positions of
+    10^6 keep 1e-7 of a turn).
     inplace: write into q and k (no gradients; refused where an element would be turned twice: expanded tensors, q and k that meet).  Gradients: q, k
     (turned back)."""
     if layout not in ("bthd", "bhtd"):
