@@ -142,3 +142,22 @@ def test_frequency_tables():
                 dict(dim=2, scaling="ntk", factor=2.0)):
         with pytest.raises(_hip.YpError):
             ops.rotary_frequencies(**bad)
+
+
+@pytest.mark.parametrize("dim,axes,base,original,factor", [(128, 1, 10000.0, 262144, 8.0), (128, 1, 10000.0, 4096, 8.0), (64, 2, 100.0, 640, 4.0), (64, 1, 500000.0, 8192, 32.0),
+                                                           (64, 2, 100.0, 1 << 20, 4.0), (64, 1, 10000.0, 4, 2.0), (64, 1, 10000.0, 6, 2.0), (2, 1, 10000.0, 640, 2.0)])
+def test_yarn_table_against_the_published_formula(dim, axes, base, original, factor):
+    """The ramp runs from floor(pair with `fast` turns) >= 0 to ceil(pair with `slow` turns) <= d - 1, wherever the last pair stands; pairs of more than `fast`
+    turns stay and pairs of fewer than `slow` are divided by the factor at every length."""
+    d, fast, slow = dim // axes, 32.0, 1.0
+    f = float(base) ** (-np.arange(d // 2) / (d / 2))
+    place = [d * math.log(original / (n * 2 * math.pi)) / (2 * math.log(base)) for n in (fast, slow)]
+    low, high = max(math.floor(place[0]), 0), min(math.ceil(place[1]), d - 1)
+    turns = original * f / (2 * math.pi)
+    want = np.empty(d // 2)
+    for j in range(d // 2):
+        r = 1.0 if turns[j] < slow else 0.0 if turns[j] > fast else (j - low) / (high - low)
+        want[j] = f[j] * (1 - r) + f[j] / factor * r
+    got, scale = ops.rotary_frequencies(dim, base, axes=axes, scaling="yarn", factor=factor, original=original)
+    # (64 bits: a handful of roundings of 2^-53 each)
+    assert got.shape == (dim // 2,) and np.allclose(got.numpy(), np.tile(want, axes), rtol=64 * 2.0 ** -53, atol=0.0) and scale == 0.1 * math.log(factor) + 1.0

@@ -111,7 +111,8 @@ def rotary_frequencies(dim, base=10000.0, axes=1, scaling=None, factor=1.0, orig
       'linear'  positions divided by factor
       'ntk'     base * factor^(dim / (dim - 2)): the slowest pair is stretched by factor, the fastest stays
       'yarn'    pairs that turn more than `fast` times over `original` positions stay, those below `slow` turns are divided by factor, a linear
-                ramp over the pairs between them; scale = 0.1 ln(factor) + 1"""
+                ramp over the pairs between them (from the whole pair below the one border to the whole pair above the other, which may
+                lie behind the last pair: the published method's `d - 1`, d = dim / axes); scale = 0.1 ln(factor) + 1"""
     if axes not in (1, 2) or dim < 2 * axes or dim % (2 * axes):
         raise _hip.YpError(f"rotary_frequencies: {dim} features over {axes} axes")
     if scaling not in (None, "linear", "ntk", "yarn") or not factor >= 1.0 or (scaling is None and factor != 1.0):
@@ -132,8 +133,10 @@ def rotary_frequencies(dim, base=10000.0, axes=1, scaling=None, factor=1.0, orig
         def pair_of(turns):                         # the (fractional) pair that makes this many turns over the original length
             return d * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-        low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), d // 2 - 1)
-        ramp = [min(max((j - low) / max(high - low, 1e-3), 0.0), 1.0) for j in range(d // 2)]
+        end = pair_of(slow)
+        low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(end), d - 1)
+        # (j > end: the first pair of a length that it does not turn over once stands on low = 0 and yet behind the ramp)
+        ramp = [1.0 if j > end else min(max((j - low) / max(high - low, 1e-3), 0.0), 1.0) for j in range(d // 2)]
         f = [v * (1.0 - r) + v / factor * r for v, r in zip(f, ramp)]
         scale = 0.1 * math.log(factor) + 1.0
     return torch.tensor(f * axes, dtype=torch.float64, device=device), scale
