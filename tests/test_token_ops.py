@@ -161,3 +161,16 @@ def test_yarn_table_against_the_published_formula(dim, axes, base, original, fac
     got, scale = ops.rotary_frequencies(dim, base, axes=axes, scaling="yarn", factor=factor, original=original)
     # (64 bits: a handful of roundings of 2^-53 each)
     assert got.shape == (dim // 2,) and np.allclose(got.numpy(), np.tile(want, axes), rtol=64 * 2.0 ** -53, atol=0.0) and scale == 0.1 * math.log(factor) + 1.0
+
+
+def test_frequency_tables_refuse_what_has_no_table():
+    inf, nan = math.inf, math.nan
+    yarn = dict(dim=8, scaling="yarn", factor=2.0)
+    for bad in (dict(dim=8, base=0.0), dict(dim=8, base=-2.0), dict(dim=8, base=nan), dict(dim=8, base=inf), dict(dim=8, base="b"), dict(dim=8.0), dict(dim="8"), dict(dim=8, axes=1.0),
+                dict(dim=8, factor=nan), dict(dim=8, scaling="linear", factor=inf), dict(dim=8, scaling="ntk", factor=inf), dict(dim=16, base=1e300, scaling="ntk", factor=1e300),
+                dict(yarn, original=-5), dict(yarn, original=inf), dict(yarn, original=nan), dict(yarn, original="x"), dict(yarn, original=64, base=1.0), dict(yarn, original=64, base=0.5),
+                dict(yarn, original=64, fast=inf), dict(yarn, original=64, slow=nan), dict(yarn, original=64, factor="y"), dict(dim=8, base=10 ** 400)):
+        with pytest.raises(_hip.YpError):
+            ops.rotary_frequencies(**bad)
+    # what was a table stays one
+    assert torch.equal(ops.rotary_frequencies(np.int64(8), 1.0)[0], torch.ones(4, dtype=torch.float64)) and ops.rotary_frequencies(8, 0.25)[0][1] == 0.25 ** -0.25

@@ -15,6 +15,7 @@ import importlib.machinery
 import importlib.util
 import ctypes as C
 import math
+import operator
 import os
 import threading
 
@@ -113,11 +114,19 @@ def rotary_frequencies(dim, base=10000.0, axes=1, scaling=None, factor=1.0, orig
       'yarn'    pairs that turn more than `fast` times over `original` positions stay, those below `slow` turns are divided by factor, a linear
                 ramp over the pairs between them (from the whole pair below the one border to the whole pair above the other, which may
                 lie behind the last pair: the published method's `d - 1`, d = dim / axes); scale = 0.1 ln(factor) + 1"""
+    try:
+        dim, axes, base, factor = operator.index(dim), operator.index(axes), float(base), float(factor)
+        original, fast, slow = None if original is None else float(original), float(fast), float(slow)
+    except (TypeError, ValueError, OverflowError) as e:
+        raise _hip.YpError(f"rotary_frequencies: {e}") from None
     if axes not in (1, 2) or dim < 2 * axes or dim % (2 * axes):
         raise _hip.YpError(f"rotary_frequencies: {dim} features over {axes} axes")
-    if scaling not in (None, "linear", "ntk", "yarn") or not factor >= 1.0 or (scaling is None and factor != 1.0):
+    if scaling not in (None, "linear", "ntk", "yarn") or not 1.0 <= factor < math.inf or (scaling is None and factor != 1.0):
         raise _hip.YpError(f"rotary_frequencies: scaling {scaling!r} by {factor}")
     d = dim // axes
+    # (the largest table value and, for 'ntk', the stretched base have to be numbers)
+    if not 0.0 < base < math.inf or abs(math.log(base)) + (math.log(factor) * 2.0 if scaling == "ntk" else 0.0) > 700.0:
+        raise _hip.YpError(f"rotary_frequencies: base {base} (stretched by {factor})")
     if scaling == "ntk":
         if d < 4:
             raise _hip.YpError("rotary_frequencies: 'ntk' needs two pairs an axis")
@@ -127,8 +136,8 @@ def rotary_frequencies(dim, base=10000.0, axes=1, scaling=None, factor=1.0, orig
     if scaling == "linear":
         f = [v / factor for v in f]
     elif scaling == "yarn":
-        if not original or not fast > slow > 0.0:
-            raise _hip.YpError("rotary_frequencies: 'yarn' needs the original length and fast > slow > 0")
+        if original is None or not 0.0 < original < math.inf or not math.inf > fast > slow > 0.0 or not base > 1.0:
+            raise _hip.YpError("rotary_frequencies: 'yarn' needs the original length, fast > slow > 0 and a base over 1")
 
         def pair_of(turns):                         # the (fractional) pair that makes this many turns over the original length
             return d * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
