@@ -856,3 +856,27 @@ def test_a_block_over_keypoint_tokens(cuda, dtype):
     for name, a, b in zip(("y", "x", *P), (got, *got_g), (want, *want_g)):
         rel = float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm())
         assert rel <= bar, (name, rel, bar)
+
+
+# ------------------------------------------------------------------------------------------------------------------ calls that other machinery watches
+def test_traced_calls_are_refused_on_the_device(cuda):
+    """Forward and backward under a tracer; under a mode that only watches, the call runs as ever."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    x, dy = make(cuda, (9, 64), torch.bfloat16, 1), make(cuda, (9, 64), torch.bfloat16, 2)
+    inv = ops.rotary_frequencies(64)[0].to(cuda)
+    for f in (lambda t: ops.layer_norm(t), lambda t: ops.dropout_add_layer_norm(t, t, p=0.5, rng=(1, 2))[0], lambda t: ops.dropout(t, 0.5, (1, 2)),
+              lambda t: ops.rotary(t.view(1, 9, 1, 64), 3, inv).view(9, 64)):
+        with pytest.raises(_hip.YpError, match="cannot be traced"):
+            torch.jit.trace(f, x)
+        with pytest.raises(_hip.YpError, match="cannot be traced"):
+            make_fx(f)(x)
+        leaf = x.clone().requires_grad_()
+        y = f(leaf)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True)[0])(dy)
+        want = torch.autograd.grad(y, leaf, dy)[0]
+        with FlopCounterMode(display=False):
+            again = f(leaf)
+            got, = torch.autograd.grad(again, leaf, dy)
+        assert torch.equal(again, y) and torch.equal(got, want)

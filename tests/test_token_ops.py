@@ -174,3 +174,25 @@ def test_frequency_tables_refuse_what_has_no_table():
             ops.rotary_frequencies(**bad)
     # what was a table stays one
     assert torch.equal(ops.rotary_frequencies(np.int64(8), 1.0)[0], torch.ones(4, dtype=torch.float64)) and ops.rotary_frequencies(8, 0.25)[0][1] == 0.25 ** -0.25
+
+
+def traced_calls(inv):
+    return {"layer_norm": lambda t: ops.layer_norm(t), "dropout_add_layer_norm": lambda t: ops.dropout_add_layer_norm(t, t)[0], "dropout": lambda t: ops.dropout(t, 0.5, (1, 2)),
+            "rotary": lambda t: ops.rotary(t.view(1, 1, *t.shape), 0, inv)}
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "dropout_add_layer_norm", "dropout", "rotary"])
+def test_traced_calls_are_refused(op):
+    """A recording would hold the empty buffers of the results and not what fills them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, inv = torch.randn(4, 8), ops.rotary_frequencies(8)[0]
+    f = traced_calls(inv)[op]
+    with pytest.raises(_hip.YpError, match="cannot be traced"):
+        torch.jit.trace(f, x)
+    with pytest.raises(_hip.YpError, match="cannot be traced"):
+        make_fx(f)(x)
+    with pytest.raises(_hip.YpError, match="cannot be traced"), FakeTensorMode(allow_non_fake_inputs=True):
+        f(x)
+    with pytest.raises(_hip.YpError, match="on the GPU"):
+        f(x)

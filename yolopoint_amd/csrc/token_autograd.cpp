@@ -4,11 +4,13 @@
 // The entry points come as addresses from the ctypes binding (init), so that this module serves whichever build of the library is loaded.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <cstdarg>
 #include <optional>
@@ -60,7 +62,18 @@ std::string shape_of(const Tensor& t) {
     return s + "]";
 }
 
+// A tracer sees the buffers that a call allocates and not the kernels that fill them: what it recorded would return memory as it was found.  (Other
+// dispatch modes -- counters, checkpointing -- run the call as it is and may stay.)
+void check_untraced(const char* what) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    bool traced = torch::jit::tracer::isTracing();
+    if (!traced && Modes::any_modes_set())
+        for (int i = 0; i < (int)c10::impl::TorchDispatchModeKey::NUM_MODE_KEYS; ++i) traced |= Modes::get_mode((c10::impl::TorchDispatchModeKey)i).has_value();
+    if (traced) fail("%s: cannot be traced (torch.jit.trace, make_fx, fake tensors): its kernels are launched, not dispatched", what);
+}
+
 void check_tensor(const char* what, const Tensor& x) {
+    check_untraced(what);
     if (!x.defined() || !x.is_cuda()) fail("%s: a tensor on the GPU is needed (there is no CPU path)", what);
     if (x.layout() != at::kStrided || type_code(x.scalar_type()) < 0) fail("%s: a dense tensor of float16, bfloat16 or float32, not %s", what, toString(x.scalar_type()));
     if (x._fw_grad(0).defined()) fail("%s: forward-mode differentiation is not offered", what);
@@ -190,6 +203,7 @@ struct NormBackward : Node {
         std::lock_guard<std::mutex> lock(mutex_);
         const int n = fused ? 4 : 3;
         variable_list out(n);
+        check_untraced(fused ? "dropout_add_layer_norm's gradient" : "layer_norm's gradient");
         Tensor dy = in[0], dz = fused ? in[1] : Tensor();
         if (!dy.defined() && !dz.defined()) return out;
         const Tensor z_ = z.unpack(shared_from_this()), w_ = weight.unpack(), stats_ = stats.unpack(), rng_ = rng.unpack();
@@ -319,6 +333,7 @@ struct DropoutBackward : Node {
     variable_list apply(variable_list&& in) override {     // gradients of (x, residual)
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(2);
+        check_untraced("dropout's gradient");
         const Tensor dy = in[0];
         if (!dy.defined()) return out;
         const Tensor rng_ = rng.unpack();
@@ -434,6 +449,7 @@ struct RotaryBackward : Node {
     variable_list apply(variable_list&& in) override {     // gradients of (q, k)
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(2);
+        check_untraced("rotary's gradient");
         const Tensor dq = task_should_compute_output(0) ? in[0] : Tensor(), dk = has_k && task_should_compute_output(1) ? in[1] : Tensor();
         const Tensor first = dq.defined() ? dq : dk, second = dq.defined() ? dk : Tensor();
         if (!first.defined()) return out;
