@@ -880,3 +880,29 @@ def test_traced_calls_are_refused_on_the_device(cuda):
             again = f(leaf)
             got, = torch.autograd.grad(again, leaf, dy)
         assert torch.equal(again, y) and torch.equal(got, want)
+
+
+def test_operands_without_memory_are_refused(cuda):
+    """A wrapper beside ordinary tensors must not pass for an operand that was not given; a tensor that torch knows to be zero is one of zeros."""
+    from test_token_ops import Wrapper
+
+    def hollow(t):
+        return Wrapper(t.shape, t.dtype, t.device)
+    x, r, w = make(cuda, (4, 8), torch.float32, 1), make(cuda, (4, 8), torch.float32, 2), make(cuda, (8,), torch.float32, 3)
+    q, at, inv, state = make(cuda, (1, 4, 2, 8), torch.float32, 4), torch.arange(4, device=cuda), ops.rotary_frequencies(8)[0].to(cuda), torch.tensor([1, 2], device=cuda)
+    for call in (lambda: ops.layer_norm(x, hollow(w)), lambda: ops.layer_norm(x, None, hollow(w)), lambda: ops.dropout(x, 0.5, hollow(state)), lambda: ops.dropout(x, 0.5, (1, 2), residual=hollow(x)),
+                 lambda: ops.dropout_add_layer_norm(x, hollow(x)), lambda: ops.dropout_add_layer_norm(x, r, hollow(w)), lambda: ops.dropout_add_layer_norm(x, r, p=0.5, rng=hollow(state)),
+                 lambda: ops.rotary(q, hollow(at), inv), lambda: ops.rotary(q, at, hollow(inv)), lambda: ops.rotary(q, at, inv, k=hollow(q)), lambda: ops.rotary(hollow(q), at, inv)):
+        with pytest.raises(_hip.YpError):
+            call()
+    zero = torch._efficientzerotensor((4, 8), device=cuda)
+    assert zero.data_ptr() == 0
+    none = torch.zeros(4, 8, device=cuda)
+    assert torch.equal(ops.dropout_add_layer_norm(x, zero)[1], x) and torch.equal(ops.dropout(zero, 0.5, (1, 2), residual=r), r) and torch.equal(ops.layer_norm(zero), none)
+    assert not ops.rotary(zero.view(1, 4, 1, 8), at, inv).any()
+    a, b = x.clone().requires_grad_(), r.clone().requires_grad_()
+    y, z = ops.dropout_add_layer_norm(a, b, p=0.5, rng=(1, 2))
+    want = torch.autograd.grad((y, z), (a, b), (none, x), retain_graph=True)
+    assert all(torch.equal(i, j) for i, j in zip(torch.autograd.grad((y, z), (a, b), (zero, x), retain_graph=True), want))
+    want = torch.autograd.grad((y, z), (a, b), (x, none), retain_graph=True)
+    assert all(torch.equal(i, j) for i, j in zip(torch.autograd.grad((y, z), (a, b), (x, zero)), want))

@@ -196,3 +196,22 @@ def test_traced_calls_are_refused(op):
         f(x)
     with pytest.raises(_hip.YpError, match="on the GPU"):
         f(x)
+
+
+class Wrapper(torch.Tensor):
+    """A tensor that says where it lies and holds nothing there, as sharded parameters do."""
+    @staticmethod
+    def __new__(cls, shape, dtype, device):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device=device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise RuntimeError(f"{func} was called on a wrapper")
+
+
+def test_tensors_without_memory_are_refused():
+    x, inv = Wrapper((4, 8), torch.float32, "cuda:0"), ops.rotary_frequencies(8)[0]
+    for call in (lambda: ops.layer_norm(x), lambda: ops.dropout(x, 0.5, (1, 2)), lambda: ops.dropout_add_layer_norm(x, x),
+                 lambda: ops.rotary(Wrapper((1, 2, 3, 8), torch.float32, "cuda:0"), 0, inv)):
+        with pytest.raises(_hip.YpError, match="memory"):
+            call()

@@ -72,20 +72,44 @@ void check_untraced(const char* what) {
     if (traced) fail("%s: cannot be traced (torch.jit.trace, make_fx, fake tensors): its kernels are launched, not dispatched", what);
 }
 
+// A tensor with elements has memory: the entry points take a missing address for an operand that was not given, so tensors without storage of their own
+// (sharded parameters and other wrappers, fake tensors) must not reach them.  (Tensors that torch knows to be zero are written out where they are read.)
+bool has_memory(const Tensor& t) {
+    if (t.numel() == 0 || t._is_zerotensor()) return true;
+    if (!t.has_storage()) return false;
+    try {
+        return t.const_data_ptr() != nullptr;
+    } catch (const c10::Error&) {
+        return false;
+    }
+}
+void check_memory(const char* what, const Tensor& t) {
+    if (!has_memory(t)) fail("%s: a tensor of shape %s holds no memory of its own (a wrapper: pass what it wraps)", what, shape_of(t).c_str());
+}
+
 void check_tensor(const char* what, const Tensor& x) {
     check_untraced(what);
     if (!x.defined() || !x.is_cuda()) fail("%s: a tensor on the GPU is needed (there is no CPU path)", what);
     if (x.layout() != at::kStrided || type_code(x.scalar_type()) < 0) fail("%s: a dense tensor of float16, bfloat16 or float32, not %s", what, toString(x.scalar_type()));
+    check_memory(what, x);
     if (x._fw_grad(0).defined()) fail("%s: forward-mode differentiation is not offered", what);
 }
 void check_beside(const char* what, const Tensor& x, const MaybeTensor& o) {
     if (o && (o->device() != x.device() || o->layout() != at::kStrided)) fail("%s: all tensors dense and on %s", what, x.device().str().c_str());
+    if (o) check_memory(what, *o);
     if (o && o->is_floating_point() && o->_fw_grad(0).defined()) fail("%s: forward-mode differentiation is not offered", what);
 }
 
 bool wants(const MaybeTensor& t) { return t && t->requires_grad(); }
 Tensor given(const MaybeTensor& t) { return t ? *t : Tensor(); }
-void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// the address of an operand: null for one that was not given, and for no other that has elements
+void* address(const Tensor& t) {
+    if (!t.defined() || t.numel() == 0) return nullptr;
+    void* p = t.has_storage() ? t.data_ptr() : nullptr;
+    if (p == nullptr) fail("a token operator was given a tensor of shape %s without memory", shape_of(t).c_str());
+    return p;
+}
 
 // gradients of gradients are refused when they are asked for, as by once_differentiable
 variable_list once(variable_list&& grads) {
@@ -97,13 +121,16 @@ variable_list once(variable_list&& grads) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- rows
-// t as it lies if it is dense, else a dense copy (also of a view that is negated when it is read, as the imaginary part of a conjugate is)
-Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+// t with its values in memory: a copy of a view that is negated when it is read (the imaginary part of a conjugate is), and of one that is known to be zero
+Tensor plain(const Tensor& t) { return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
+
+// t as it lies if it is dense, else a dense copy
+Tensor dense(const Tensor& t) { return t.defined() ? plain(t).contiguous() : t; }
 
 // x with rows of one distance where they lie, anything else through a dense copy
 struct Rows { Tensor t; int64_t stride; };
 Rows rows_of(const Tensor& t) {
-    const Tensor x = t.resolve_neg();
+    const Tensor x = plain(t);
     const int64_t D = x.size(-1);
     if (x.is_contiguous()) return {x, D};
     if (D == 1 || x.stride(-1) == 1) {
@@ -138,7 +165,7 @@ void check_norm(const char* what, const Tensor& x, const MaybeTensor& w, const M
 
 void check_drop(const char* what, const Tensor& x, double p, const MaybeTensor& rng) {
     if (!(p >= 0.0 && p <= 1.0)) fail("%s: a rate of 0 to 1, not %g", what, p);
-    if (rng && (rng->scalar_type() != at::kLong || rng->dim() != 1 || rng->size(0) != 2 || !rng->is_contiguous() || rng->is_neg() || rng->device() != x.device()))
+    if (rng && (rng->scalar_type() != at::kLong || rng->dim() != 1 || rng->size(0) != 2 || !rng->is_contiguous() || rng->is_neg() || rng->device() != x.device() || !has_memory(*rng)))
         fail("%s: rng as a tensor is int64 [seed, offset] on %s", what, x.device().str().c_str());
 }
 
@@ -157,7 +184,7 @@ NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& w
     if (residual.defined()) {
         rr = rows_of(residual);
         r.z = at::empty(x.sizes(), r.y.options());
-        d.res = rr.t.data_ptr();
+        d.res = address(rr.t);
         d.res_stride = rr.stride;
         d.z = r.z.data_ptr();
     }
@@ -166,7 +193,7 @@ NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& w
         d.mean = (float*)r.stats.data_ptr();
         d.rstd = d.mean + rows;
     }
-    d.x = xr.t.data_ptr();
+    d.x = address(xr.t);
     d.x_stride = xr.stride;
     d.y = r.y.data_ptr();
     d.weight = address(w);
@@ -228,12 +255,12 @@ struct NormBackward : Node {
                 ws = at::empty({(int64_t)d.workspace_bytes}, options.dtype(at::kByte));
                 d.workspace = ws.data_ptr();
             }
-            if (dz.defined()) { dzr = rows_of(dz); d.dz = dzr.t.data_ptr(); d.dz_stride = dzr.stride; }
-            d.x = zr.t.data_ptr();
+            if (dz.defined()) { dzr = rows_of(dz); d.dz = address(dzr.t); d.dz_stride = dzr.stride; }
+            d.x = address(zr.t);
             d.x_stride = zr.stride;
-            d.dy = dyr.t.data_ptr();
+            d.dy = address(dyr.t);
             d.dy_stride = dyr.stride;
-            d.mean = (float*)stats_.data_ptr();
+            d.mean = (float*)address(stats_);
             d.rstd = d.mean + rows;
             d.weight = address(w);
             d.dres = dres.data_ptr();
@@ -317,7 +344,7 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const MaybeTe
 Tensor drop_launch(const Tensor& x, const Tensor& residual, const Dropping& drop, const Tensor& rng) {
     const Tensor xc = dense(x), rc = dense(residual);
     Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    check(lib.dropout(xc.data_ptr(), address(rc), y.data_ptr(), x.numel(), type_code(x.scalar_type()), drop.p, drop.seed, drop.offset, (const int64_t*)address(rng), stream_of(x)));
+    check(lib.dropout(address(xc), address(rc), y.data_ptr(), x.numel(), type_code(x.scalar_type()), drop.p, drop.seed, drop.offset, (const int64_t*)address(rng), stream_of(x)));
     return y;
 }
 
@@ -391,7 +418,7 @@ void strides_of(const Tensor& x, bool heads_first, int64_t (&s)[3]) {
 void turn_launch(const Tensor& q, const Tensor& k, const Tensor& q_out, const Tensor& k_out, const Tensor& positions, const Tensor& inv_freq, const Turn& how, bool inverse) {
     YpRotaryDesc d{};
     const bool hf = how.heads_first;
-    d.q = q.data_ptr();
+    d.q = address(q);
     d.q_out = q_out.data_ptr();
     strides_of(q, hf, d.q_stride);
     strides_of(q_out, hf, d.q_out_stride);
@@ -399,7 +426,7 @@ void turn_launch(const Tensor& q, const Tensor& k, const Tensor& q_out, const Te
     d.T = (int32_t)tokens_of(q, hf);
     d.Hq = (int32_t)heads_of(q, hf);
     if (k.defined()) {
-        d.k = k.data_ptr();
+        d.k = address(k);
         d.k_out = k_out.data_ptr();
         strides_of(k, hf, d.k_stride);
         strides_of(k_out, hf, d.k_out_stride);
@@ -407,10 +434,10 @@ void turn_launch(const Tensor& q, const Tensor& k, const Tensor& q_out, const Te
     }
     d.D = (int32_t)q.size(3);
     d.R = 2 * (int32_t)inv_freq.numel();
-    d.inv_freq = (const double*)inv_freq.data_ptr();
+    d.inv_freq = (const double*)address(inv_freq);
     if (positions.defined()) {
         const int64_t n = positions.dim() - (how.axes == 2 ? 1 : 0);        // [T] or [B, T], behind it the axes
-        d.positions = positions.data_ptr();
+        d.positions = address(positions);
         d.position_type = positions.scalar_type() == at::kLong ? YP_POS_I64 : positions.scalar_type() == at::kInt ? YP_POS_I32 : YP_POS_F32;
         d.position_stride[0] = n == 2 && positions.size(0) != 1 ? positions.stride(0) : 0;
         d.position_stride[1] = positions.stride(n - 1);
@@ -425,7 +452,7 @@ void turn_launch(const Tensor& q, const Tensor& k, const Tensor& q_out, const Te
     check(lib.rotary(&d, stream_of(q)));
 }
 
-Tensor feature_dense(const Tensor& x) { return x.defined() && x.stride(3) == 1 && !x.is_neg() ? x : dense(x); }
+Tensor feature_dense(const Tensor& x) { return x.defined() && x.stride(3) == 1 && !x.is_neg() && !x._is_zerotensor() ? x : dense(x); }
 
 std::pair<Tensor, Tensor> turned(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, const Turn& how, bool inverse) {
     const Tensor qd = feature_dense(q), kd = feature_dense(k);
@@ -534,11 +561,11 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
         }
     }
     const c10::DeviceGuard guard(q.device());
-    const Tensor k_ = given(k), positions_ = positions ? positions->resolve_neg() : Tensor();
+    const Tensor k_ = given(k), positions_ = positions ? plain(*positions) : Tensor();
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || wants(k));
     if (inplace) {
         if (grad) fail("rotary: no gradients in place");
-        if (q.stride(3) != 1 || q.is_neg() || (k && (k->stride(3) != 1 || k->is_neg()))) fail("rotary: dense features in place");
+        if (q.stride(3) != 1 || q.is_neg() || q._is_zerotensor() || (k && (k->stride(3) != 1 || k->is_neg() || k->_is_zerotensor()))) fail("rotary: dense features in place");
         if (q.numel() + (k ? k->numel() : 0) == 0) return {q, k};
         if (!apart(q) || (k && (!apart(*k) || !separate(q, *k, heads_first)))) fail("rotary: q and k hold each element once in place");
         q.unsafeGetTensorImpl()->bump_version();            // (refuses an inference tensor outside inference mode)

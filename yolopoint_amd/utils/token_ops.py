@@ -7,7 +7,8 @@ neighbour (models/model_wrap.py:434-476).
 All of them: float16, bfloat16 or float32 tensors on the GPU, any leading dimensions, rows that may start on any element (slices of wider tensors are read
 in place where their rows have one distance, else copied first); sums, statistics and angles in 32 bits or more, results rounded once;
 launches on the current stream; differentiable once (a second differentiation raises).  CPU tensors, mixed devices, other types or shapes raise YpError,
-and so does a call that is traced (torch.jit.trace, make_fx, fake tensors: the recording would hold the buffers without the kernels).
+and so do tensors without memory of their own (wrappers such as sharded parameters) and a call that is traced (torch.jit.trace, make_fx, fake tensors:
+the recording would hold the buffers without the kernels).
 
 A captured graph replays the kernels on the same addresses: `rng` as a device tensor lets every replay draw another mask.  A backward pass may be
 captured with its forward pass; leaves that an eager graph still holds must not take part in it.
