@@ -906,3 +906,14 @@ def test_operands_without_memory_are_refused(cuda):
     assert all(torch.equal(i, j) for i, j in zip(torch.autograd.grad((y, z), (a, b), (zero, x), retain_graph=True), want))
     want = torch.autograd.grad((y, z), (a, b), (x, none), retain_graph=True)
     assert all(torch.equal(i, j) for i, j in zip(torch.autograd.grad((y, z), (a, b), (x, zero)), want))
+
+
+def test_a_state_that_is_not_read_may_move_on(cuda):
+    """Rates of 0 (or below half a step) draw nothing: the state may be written between forward and backward."""
+    x, r, dy = (make(cuda, (7, 24), torch.bfloat16, i) for i in range(3))
+    for p in (0.0, 1e-6):
+        for f in (lambda a, s: ops.dropout(a, p, s), lambda a, s: ops.dropout(a, p, s, residual=r), lambda a, s: ops.dropout_add_layer_norm(a, r, p=p, rng=s)[1]):
+            state, leaf = torch.tensor([3, 4], device=cuda), x.clone().requires_grad_()
+            y = f(leaf, state)
+            state[1] += 1
+            assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], dy)

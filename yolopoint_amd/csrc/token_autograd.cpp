@@ -148,7 +148,11 @@ Rows rows_of(const Tensor& t) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- layer norm
-struct Dropping { double p = 0.0; uint64_t seed = 0, offset = 0; };
+struct Dropping {
+    double p = 0.0;
+    uint64_t seed = 0, offset = 0;
+    bool any() const { return p * 65536.0 + 0.5 >= 1.0; }  // (the applied rate, in steps of 2^-16)
+};
 
 void check_norm(const char* what, const Tensor& x, const MaybeTensor& w, const MaybeTensor& b, double eps) {
     const int widest = lib.norm_max_width(type_code(x.scalar_type()));
@@ -244,7 +248,7 @@ struct NormBackward : Node {
             const Tensor w = dense(w_);
             const auto options = z_.options().memory_format(at::MemoryFormat::Contiguous);
             const Tensor dres = at::empty(z_.sizes(), options);
-            const bool drops = drop.p * 65536.0 + 0.5 >= 1.0;
+            const bool drops = drop.any();
             Tensor dx, dw, db, ws;
             YpLayerNormDesc d{};
             if (drops) { dx = at::empty(z_.sizes(), options); d.dx = dx.data_ptr(); }
@@ -335,7 +339,7 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const MaybeTe
         node->z = SavedVariable(r.z, true);
         node->weight = SavedVariable(w, false);
         node->stats = SavedVariable(r.stats, false);
-        node->rng = SavedVariable(state, false);
+        if (drop.any()) node->rng = SavedVariable(state, false);     // (a state that is not read may move on)
     }
     return {r.y, r.z};
 }
@@ -392,7 +396,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
         std::shared_ptr<DropoutBackward> node(new DropoutBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x, r));
         node->drop = drop;
-        node->rng = SavedVariable(state, false);
+        if (drop.any()) node->rng = SavedVariable(state, false);
         torch::autograd::set_history(y, node);
     }
     return y;
