@@ -725,7 +725,7 @@ typedef struct YpRotaryDesc {
     const double* inv_freq;
     int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3], position_stride[3];
     int64_t start;
-    int32_t B, T, Hq, Hk, D, R;      /* B * T < 2^31, D <= 1024, R even */
+    int32_t B, T, Hq, Hk, D, R;      /* B * T < 2^31, Hq + Hk <= 2^30, D <= 1024, R even */
     int32_t dtype, position_type, axes, interleaved, inverse;
     float scale;
 } YpRotaryDesc;

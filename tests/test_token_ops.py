@@ -215,3 +215,12 @@ def test_tensors_without_memory_are_refused():
                  lambda: ops.rotary(Wrapper((1, 2, 3, 8), torch.float32, "cuda:0"), 0, inv)):
         with pytest.raises(_hip.YpError, match="memory"):
             call()
+
+
+def test_rotary_refuses_head_counts_past_32_bits():
+    """A thread steps over the heads in 32 bits: a sum of heads near 2^31 would wrap to heads before the first."""
+    l = _hip.lib()
+    for Hq, Hk, B, T in (((1 << 30) + 1, 0, 1, 1), (1 << 30, 1, 1, 1), ((1 << 30) - 1, (1 << 30) - 1, 1, 1), ((1 << 31) - 1, (1 << 31) - 1, 1, 1), ((1 << 31) - 1, 1, 1, 4),
+                         (1 << 30, 0, 1 << 10, 1 << 20)):
+        d = _hip.YpRotaryDesc(q=64, k=64, q_out=64, k_out=64, positions=64, inv_freq=64, B=B, T=T, Hq=Hq, Hk=Hk, D=2, R=2, axes=1, scale=1.0)
+        assert l.yp_rotary(C.byref(d), None) == -1 and b"heads" in l.yp_last_error()

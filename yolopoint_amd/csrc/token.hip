@@ -171,6 +171,8 @@ extern "C" int yp_rotary(const YpRotaryDesc* d, void* stream) {
     YP_REQUIRE(d != nullptr, "yp_rotary: no descriptor");
     YP_REQUIRE(d->dtype == YP_F16 || d->dtype == YP_BF16 || d->dtype == YP_F32, "yp_rotary: type %d", d->dtype);
     YP_REQUIRE(d->B >= 0 && d->T >= 0 && d->Hq >= 0 && d->Hk >= 0 && (int64_t)d->B * d->T < (int64_t)1 << 31, "yp_rotary: %d x %d tokens, %d + %d heads", d->B, d->T, d->Hq, d->Hk);
+    // (a thread's next head is its head + up to 256, in 32 bits)
+    YP_REQUIRE((int64_t)d->Hq + d->Hk <= (int64_t)1 << 30 && (int64_t)d->B * d->T * ((int64_t)d->Hq + d->Hk) < (int64_t)1 << 53, "yp_rotary: %d + %d heads of %d x %d tokens", d->Hq, d->Hk, d->B, d->T);
     YP_REQUIRE(d->D >= 2 && d->D <= 1024 && d->R >= 2 && d->R <= d->D && d->R % 2 == 0, "yp_rotary: %d of %d features", d->R, d->D);
     YP_REQUIRE((d->axes == 1 || d->axes == 2) && d->R / 2 % d->axes == 0, "yp_rotary: %d axes over %d pairs", d->axes, d->R / 2);
     YP_REQUIRE(d->position_type == YP_POS_I32 || d->position_type == YP_POS_I64 || d->position_type == YP_POS_F32, "yp_rotary: positions of type %d", d->position_type);
