@@ -917,3 +917,38 @@ def test_a_state_that_is_not_read_may_move_on(cuda):
             y = f(leaf, state)
             state[1] += 1
             assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], dy)
+
+
+def test_rotary_in_place_beside_each_other(cuda):
+    """q and k of one tensor, side by side at any depth, share no element: turned in place; what meets stays refused."""
+    B, T, H, D = 2, 5, 4, 16
+    inv, at = ops.rotary_frequencies(D)[0].to(cuda), torch.arange(T, device=cuda) + 7
+
+    def turned(joint, q, k, layout="bthd"):
+        """q, k: functions of the joint tensor"""
+        want = ops.rotary(q(joint), at, inv, k=k(joint), layout=layout)
+        rest = joint.clone()
+        q(rest).zero_(), k(rest).zero_()
+        ops.rotary(q(joint), at, inv, k=k(joint), layout=layout, inplace=True)
+        assert torch.equal(q(joint), want[0]) and torch.equal(k(joint), want[1])
+        q(joint).zero_(), k(joint).zero_()
+        assert torch.equal(joint, rest)                                              # nothing but q and k was written
+    for i, j in ((0, 1), (1, 0), (2, 0), (1, 2)):
+        turned(make(cuda, (B, T, H, 3, D), torch.bfloat16, 1), lambda t: t[..., i, :], lambda t: t[..., j, :])            # beside each other in a head
+        turned(make(cuda, (B, T, 3, H, D), torch.float32, 2), lambda t: t[:, :, i], lambda t: t[:, :, j])                # in a token
+        turned(make(cuda, (T, B, 3, H, D), torch.bfloat16, 3), lambda t: t[:, :, i].transpose(0, 1), lambda t: t[:, :, j].transpose(0, 1))
+        turned(make(cuda, (B, 3, H, T, D), torch.float16, 4), lambda t: t[:, i], lambda t: t[:, j], "bhtd")              # in a batch entry
+        turned(make(cuda, (B, H, T, 3, D), torch.float16, 5), lambda t: t[..., i, :], lambda t: t[..., j, :], "bhtd")
+    turned(make(cuda, (B, T, 2, 3, D), torch.bfloat16, 6), lambda t: t[:, :, 0:1, :2].flatten(2, 3), lambda t: t[:, :, 1, 2:], "bthd")     # head numbers 2 and 1
+    turned(make(cuda, (B, T, H, 3 * D), torch.bfloat16, 7), lambda t: t[:, :, :, 3:3 + D], lambda t: t[:, :, :2, 2 * D:])                  # every head of q, the first two of k
+    odd = make(cuda, (B, T, H, 3 * D), torch.bfloat16, 8)
+    clean = odd.clone()
+    for q, k in ((odd[..., :D], odd[..., D // 2:D // 2 + D]), (odd[..., :D], odd[..., :D]), (odd[:, :, :2, :D], odd[:, :, 1:3, :D]), (odd[..., D:2 * D], odd[:, :, 1:, D:2 * D]),
+                 (odd[..., 2 * D:], odd.flatten()[3 * D - 8:][:B * T * H * 2 * D].view(B, T, H, 2 * D)[..., :D])):
+        with pytest.raises(_hip.YpError):
+            ops.rotary(q, at, inv, k=k, inplace=True)
+    assert torch.equal(odd, clean)
+    q, k = odd[:, :, :0, :D], odd[..., :D]                                           # no head of q: nothing to meet
+    want = ops.rotary(k, at, inv)
+    ops.rotary(q, at, inv, k=k, inplace=True)
+    assert torch.equal(k, want)

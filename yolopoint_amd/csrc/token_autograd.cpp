@@ -510,26 +510,39 @@ bool apart(const Tensor& t) {
     return true;
 }
 
-// q and k share no element: their memory does not meet, or they are parts of one tensor beside each other in every batch entry or every token
-bool separate(const Tensor& q, const Tensor& k, bool heads_first) {
-    auto reach = [](const Tensor& t, std::initializer_list<int64_t> dims) {
+// q and k share no element: their memory does not meet, or they are parts of one tensor that stand beside each other in every batch entry, token or head.
+// Of their dimensions some are walked by both with the same strides; what one step of those spans holds the one's remaining dimensions and behind them
+// the other's.  Every choice of common dimensions is tried.
+bool separate(const Tensor& q, const Tensor& k) {
+    if (q.numel() == 0 || k.numel() == 0) return true;
+    const char *a = (const char*)q.data_ptr(), *b = (const char*)k.data_ptr();
+    const Tensor &low = a <= b ? q : k, &high = a <= b ? k : q;
+    const int64_t size = q.element_size(), bytes = a <= b ? b - a : a - b;
+    auto reach = [](const Tensor& t, int common) {
         int64_t n = 1;
-        for (int64_t i : dims) n += (t.size(i) - 1) * t.stride(i);
+        for (int i = 0; i < 4; ++i)
+            if (!(common >> i & 1)) n += (t.size(i) - 1) * t.stride(i);
         return n;
     };
-    const char *a = (const char*)q.data_ptr(), *b = (const char*)k.data_ptr();
-    const int64_t size = q.element_size();
-    if (a + reach(q, {0, 1, 2, 3}) * size <= b || b + reach(k, {0, 1, 2, 3}) * size <= a) return true;
-    const Tensor &low = a <= b ? q : k, &high = a <= b ? k : q;
-    const int64_t bytes = a <= b ? b - a : a - b, shift = bytes / size;
+    if (reach(low, 0) * size <= bytes) return true;
     if (bytes % size) return false;
-    const int64_t token = heads_first ? 2 : 1, head = heads_first ? 1 : 2;
-    const bool one_batch = q.size(0) == 1, one_token = q.size(token) == 1;
-    if (!one_batch && q.stride(0) != k.stride(0)) return false;
-    if (reach(low, {1, 2, 3}) <= shift && (one_batch || shift + reach(high, {1, 2, 3}) <= q.stride(0))) return true;
-    if (!one_token && q.stride(token) != k.stride(token)) return false;
-    const int64_t both = shift + reach(high, {head, 3}), row = one_token ? both : (q.size(token) - 1) * q.stride(token) + both;
-    return reach(low, {head, 3}) <= shift && (one_token || both <= q.stride(token)) && (one_batch || row <= q.stride(0));
+    for (int common = 1; common < 8; ++common) {            // (never the features: a run of them is the smallest part)
+        std::vector<std::pair<int64_t, int64_t>> steps;
+        bool fits = reach(low, common) <= bytes / size;
+        for (int i = 0; i < 3; ++i) {
+            if (!(common >> i & 1) || std::max(q.size(i), k.size(i)) == 1) continue;
+            fits = fits && q.stride(i) == k.stride(i);
+            steps.emplace_back(q.stride(i), std::max(q.size(i), k.size(i)));
+        }
+        std::sort(steps.begin(), steps.end());
+        int64_t covered = bytes / size + reach(high, common);
+        for (auto& st : steps) {
+            fits = fits && st.first >= covered;
+            covered += (st.second - 1) * st.first;
+        }
+        if (fits) return true;
+    }
+    return false;
 }
 
 std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, const MaybeTensor& positions, int64_t start, const Tensor& inv_freq, bool interleaved, bool heads_first,
@@ -571,7 +584,7 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
         if (grad) fail("rotary: no gradients in place");
         if (q.stride(3) != 1 || q.is_neg() || q._is_zerotensor() || (k && (k->stride(3) != 1 || k->is_neg() || k->_is_zerotensor()))) fail("rotary: dense features in place");
         if (q.numel() + (k ? k->numel() : 0) == 0) return {q, k};
-        if (!apart(q) || (k && (!apart(*k) || !separate(q, *k, heads_first)))) fail("rotary: q and k hold each element once in place");
+        if (!apart(q) || (k && (!apart(*k) || !separate(q, *k)))) fail("rotary: q and k hold each element once in place");
         q.unsafeGetTensorImpl()->bump_version();            // (refuses an inference tensor outside inference mode)
         if (k) k_.unsafeGetTensorImpl()->bump_version();
         turn_launch(q, k_, q, k_, positions_, inv_freq, how, false);
