@@ -952,3 +952,63 @@ def test_rotary_in_place_beside_each_other(cuda):
     want = ops.rotary(k, at, inv)
     ops.rotary(q, at, inv, k=k, inplace=True)
     assert torch.equal(k, want)
+
+
+# ------------------------------------------------------------------------------------------------------------------ rows far from zero
+def far_rows(D, dt, seed=1):
+    """Rows whose values say little beside their mean: constant ones, ones that leave their constant in one place, steps of the type around 1024."""
+    step = torch.finfo(dt).eps
+    g = torch.Generator().manual_seed(seed + D)
+    x = torch.empty(10, D, dtype=torch.float64)
+    for i, v in enumerate((13696.0, -13696.0, 1368.0, 7.25, 40000.0, 0.0)):
+        x[i] = v
+    x[6] = 13696.0
+    x[6, D // 2] += 8192 * step
+    x[7] = 1368.0
+    x[7, -1] -= 1024 * step
+    x[8:] = 1024.0 * (1.0 + step * torch.randint(0, 3, (2, D), generator=g).double())
+    return x.to(dt)
+
+
+def centred_error(x, eps):
+    """What x - mean and 1 / deviation may be off by, (in deviations, relative): the mean is a sum of at most 30 roundings, and their result is summed and
+    taken off with at most 30 again, so that a rounding of the mean's size enters in its square only."""
+    n = 32 * 2.0 ** -24
+    _, mean, rstd, xhat = O.layer_norm(x, None, None, eps)
+    first = n * x.double().abs().mean(-1, keepdim=True)
+    return n * ((x.double() - mean).abs().mean(-1, keepdim=True) + first) * rstd, n * (1.0 + 2.0 * (first * rstd).square()) + 8 * 2.0 ** -24
+
+
+FAR_WIDTHS = [1, 7, 28, 60, 100, 777, 1000, 1091, 4100, 9000, 12345]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", FAR_WIDTHS)
+def test_layer_norm_of_rows_that_hardly_vary(cuda, D, dtype):
+    """The rounding of the mean must not become the result where eps alone makes the deviation."""
+    dt = TYPES[dtype]
+    x, w, b = far_rows(D, dt), make(cuda, (D,), torch.float32, 3), make(cuda, (D,), torch.float32, 4)
+    shift, scale = centred_error(x, 1e-5)
+    _, _, _, xhat = O.layer_norm(x, None, None, 1e-5)
+    off = shift + xhat.abs() * scale
+    near(ops.layer_norm(x.to(cuda)), xhat, 0.0, off)
+    wc, bc = w.cpu().double(), b.cpu().double()
+    near(ops.layer_norm(x.to(cuda), w, b), xhat * wc + bc, 0.0, off * wc.abs() + 2 * 2.0 ** -24 * ((xhat * wc).abs() + bc.abs()))
+    y, z = ops.dropout_add_layer_norm(torch.zeros_like(x).to(cuda), x.to(cuda))
+    assert torch.equal(z.cpu(), x)
+    near(y, xhat, 0.0, off)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [2, 60, 777, 5000, 16384])
+def test_layer_norm_of_a_constant_that_one_value_leaves(cuda, D, dtype):
+    """The lone value is far below the others, so that no fp32 sum holds all digits: bf16, which takes the exact sum's remainder for the rounding of the
+    mean, may be off by the sum's own rounding (30 steps of the mean, whose size is sqrt(D) deviations at the most)."""
+    dt = TYPES[dtype]
+    x = torch.full((3, D), 13696.0, dtype=torch.float64)
+    x[0, 0], x[1, D // 2], x[2, -1] = 2.0 ** -9 * 1.5, -(2.0 ** -7), 0.0
+    x = x.to(dt)
+    shift, scale = centred_error(x, 1e-5)
+    _, _, rstd, xhat = O.layer_norm(x, None, None, 1e-5)
+    sums = 32 * 2.0 ** -24 * x.double().abs().mean(-1, keepdim=True) * rstd if dtype == "bf16" else 0.0
+    near(ops.layer_norm(x.to(cuda)), xhat, 0.0, shift + xhat.abs() * scale + sums)

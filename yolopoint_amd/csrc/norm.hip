@@ -10,7 +10,7 @@ struct LnFwd {
     float *mean, *rstd;
     int64_t rows, xs, rs;
     int D;
-    float eps;
+    float eps, width, inv_width;                    // D and 1 / D (as arguments: no register of the lanes)
     bool w32;
     unsigned long long seed, offset;
     const int64_t* rng;
@@ -18,23 +18,27 @@ struct LnFwd {
     float scale;
 };
 
-// mean = sum x / D;  var = sum (x - mean)^2 / D;  y = (x - mean) / sqrt(var + eps) w + b.  Behind the mean, delta = sum (x - mean) / D is what rounding
-// left of it, and is taken off as well: a fp32 row of mean 4096 and deviation 1 keeps 1e-7 instead of 1e-3, a f16 row of mean 1000 and deviation 1/4
-// (one step of its type) 1e-7 instead of its half step.  bf16 rows have no such digits (a deviation of one step is 2^-8 of the mean, the mean's
-// rounding 2^-24 of it), and do without the second sum (two of some twenty instructions a value).
+// mean = sum x / D;  var = sum (x - mean)^2 / D;  y = (x - mean) / sqrt(var + eps) w + b.  Behind the mean, delta is what rounding left of it, and is taken
+// off as well: where a row hardly varies (a constant one has rstd = 316), that rounding would become the result.
+//   f32, f16   delta = sum (x - mean) / D: a fp32 row of mean 4096 and deviation 1 keeps 1e-7 instead of 1e-3, a f16 row of mean 1000 and deviation 1/4 (one
+//              step of its type) 1e-7 instead of its half step
+//   bf16       delta = (sum x - mean D) / D, what the division left, for nothing a value (the sum over x - mean takes 10 % at 1091 features): the sum itself
+//              is exact in 24 bits while no value is below 2^-16 D of the largest, as 8 bits a value and D <= 2^14 of them fit.  Where one is, it stands
+//              apart from the largest, the deviation is half of that / sqrt(D) at least, and the sum's rounding moves y by 4e-4 at the most.
+// (16-bit rows over several waves: held to the registers of five waves a SIMD, which the compiler misses by three with dropout at odd widths: 4100 features
+// 143 us against 170.)
 // The next row is on its way while this one is worked on (the first before the weights are read): its registers are not touched before its turn, or the
 // wait for them would stand right behind the loads.
 // Measured, 128 MiB a tensor: 44 - 60 us for widths 16 .. 16384 (4.5 - 6.2 TB/s), with residual and dropout 100 - 130 us (4.1 - 5.4; a large copy: 5.2 - 5.4);
 // widths just over a border with dropout are bound by their instructions (bf16 4100: 142 us, 4099: 158).
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
-__global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
+__global__ __launch_bounds__(G ? 256 : 1024, G == 0 && sizeof(T) == 2 ? 5 : 1) void ln_fwd_kernel(const LnFwd a) {
     constexpr int N = Vec<T>::N, NC = E / N, ROWS = G ? 256 / G : 1;
     constexpr bool FINE = !__is_same(T, __bf16);
     __shared__ float2 sh[2][16];
     const T *x = (const T*)a.x, *res = (const T*)a.res;
     T *z = (T*)a.z, *y = (T*)a.y;
     const int threads = G ? G : blockDim.x, t = G ? threadIdx.x % G : threadIdx.x;
-    const float inv_d = 1.0f / (float)a.D;
     const Drop d = drop_state(a.seed, a.offset, a.rng, a.threshold, a.scale);
     int c[NC];
 #pragma unroll
@@ -75,7 +79,7 @@ __global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
         for (int k = 0; k < NC; ++k)
 #pragma unroll
             for (int j = 0; j < N; ++j) { f[k][j] = (float)v[k].e[j]; s1 += f[k][j]; }
-        const float mean = row_sum<G>(s1, sh[0]) * inv_d;
+        const float sum = row_sum<G>(s1, sh[0]), mean = sum * a.inv_width;
         s1 = 0.f;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -90,19 +94,16 @@ __global__ __launch_bounds__(G ? 256 : 1024) void ln_fwd_kernel(const LnFwd a) {
         }
         if constexpr (FINE) row_sum2<G>(s1, s2, sh[1]);
         else s2 = row_sum<G>(s2, sh[1]);
-        const float delta = FINE ? s1 * inv_d : 0.f;
-        float var = s2 * inv_d;
-        if constexpr (FINE) {
-            var = fmaf(-delta, delta, var);
-            var = var < 0.f ? 0.f : var;            // (not fmaxf: a NaN stays one)
-        }
+        const float delta = (FINE ? s1 : fmaf(-mean, a.width, sum)) * a.inv_width;
+        float var = fmaf(-delta, delta, s2 * a.inv_width);
+        var = var < 0.f ? 0.f : var;                // (not fmaxf: a NaN stays one)
         const float rstd = rsqrtf(var + a.eps), shift = -delta * rstd;
         if (a.mean != nullptr && t == 0) { a.mean[row] = mean + delta; a.rstd[row] = rstd; }
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
             float o[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) o[j] = fmaf(FINE ? fmaf(f[k][j], rstd, shift) : f[k][j] * rstd, w[k][j], b[k][j]);
+            for (int j = 0; j < N; ++j) o[j] = fmaf(fmaf(f[k][j], rstd, shift), w[k][j], b[k][j]);
             store_vec<T, TAIL>(y + row * a.D, c[k], a.D, to_vec<T>(o));
         }
     }
@@ -153,7 +154,7 @@ extern "C" int yp_layer_norm_fwd(const YpLayerNormDesc* d, void* stream) {
     YP_REQUIRE(drop_parameters(d->p, &a.threshold, &a.scale), "yp_layer_norm_fwd: a dropout rate of %g", d->p);
     YP_REQUIRE(d->res != nullptr || a.threshold == 0, "yp_layer_norm_fwd: dropout needs a residual");
     a.x = d->x; a.res = d->res; a.weight = d->weight; a.bias = d->bias; a.z = d->z; a.y = d->y; a.mean = d->mean; a.rstd = d->rstd;
-    a.rows = d->rows; a.xs = d->x_stride; a.rs = d->res_stride; a.D = d->D; a.eps = d->eps; a.w32 = d->wdtype == YP_F32;
+    a.rows = d->rows; a.xs = d->x_stride; a.rs = d->res_stride; a.D = d->D; a.eps = d->eps; a.width = (float)d->D; a.inv_width = 1.0f / a.width; a.w32 = d->wdtype == YP_F32;
     a.seed = d->seed; a.offset = d->offset; a.rng = d->rng;
     hipStream_t st = (hipStream_t)stream;
     const bool res = d->res != nullptr, drop = a.threshold != 0;
