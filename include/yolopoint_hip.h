@@ -675,8 +675,10 @@ int yp_mnn_match(const float* d1, int N1, const float* d2, int N2, int D, float 
  * write are dense [rows][D].
  *   forward   z = x, or with `res`: z = res + dropout(x), one fp32 multiply-add, rounded to dtype (written to `z`);
  *             y = (z - mean) * rstd * weight + bias with mean / rstd of the stored z (weight NULL: 1, bias NULL: 0).
- *             mean, rstd: fp32 [rows], both NULL when no backward pass follows.
- *   backward  x = the z of the forward pass, mean / rstd as it wrote them, dy = gradient of y, dz = gradient of z (NULL: none).
+ *             mean, rstd: fp32 [rows], both NULL when no backward pass follows.  Or `stats` in their place: fp32 [rows][3], mean | rstd | what the
+ *             nearest fp32 number leaves of the mean.
+ *   backward  x = the z of the forward pass, mean / rstd (or stats) as it wrote them, dy = gradient of y, dz = gradient of z (NULL: none).  With
+ *             stats the gradients are as exact as y on rows far from zero; without, they carry half a step of the mean, times rstd.
  *             dres = gradient of res (of x without a residual); dx = gradient of x, written where p > 0 only (it equals dres otherwise).
  *             dweight, dbias in wdtype, each may be NULL; they need the workspace of yp_layer_norm_bwd_workspace_bytes (both NULL: none).
  *             Two passes over the same inputs give the same bits.
@@ -697,6 +699,7 @@ typedef struct YpLayerNormDesc {
     float eps;
     int32_t D;                       /* 1 .. yp_layer_norm_max_width(dtype) */
     int32_t dtype, wdtype;
+    float* stats;
 } YpLayerNormDesc;
 int yp_layer_norm_max_width(int dtype);
 int yp_layer_norm_fwd(const YpLayerNormDesc* d, void* stream);

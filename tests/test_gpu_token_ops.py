@@ -1012,3 +1012,84 @@ def test_layer_norm_of_a_constant_that_one_value_leaves(cuda, D, dtype):
     _, _, rstd, xhat = O.layer_norm(x, None, None, 1e-5)
     sums = 32 * 2.0 ** -24 * x.double().abs().mean(-1, keepdim=True) * rstd if dtype == "bf16" else 0.0
     near(ops.layer_norm(x.to(cuda)), xhat, 0.0, shift + xhat.abs() * scale + sums)
+
+
+def centred_backward(x, w, dy, eps):
+    """-> (dx, error), (dweight, error) on rows far from zero: xhat's own error as in centred_error, sums of 32 roundings, some eight operations a value."""
+    u = 2.0 ** -24
+    shift, scale = centred_error(x, eps)
+    _, _, rstd, xhat = O.layer_norm(x, None, None, eps)
+    dx, dw, _ = O.layer_norm_backward(x, w, dy, eps)
+    ex = shift + xhat.abs() * scale
+    h = (dy.double() * w.double()).abs()
+    m1, m2, moved = h.mean(-1, keepdim=True), (h * xhat.abs()).mean(-1, keepdim=True), (h * ex).mean(-1, keepdim=True)
+    terms = h + m1 + xhat.abs() * m2
+    dx_error = rstd * (xhat.abs() * (32 * u * m2 + moved) + ex * (m2 + moved) + 32 * u * m1 + (8 * u + scale) * terms)
+    dw_error = (dy.double().abs() * (ex + 2 * F32 * xhat.abs())).sum(0)
+    return (dx, dx_error), (dw, dw_error)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", FAR_WIDTHS)
+def test_layer_norm_backward_of_rows_that_hardly_vary(cuda, D, dtype):
+    """The backward pass has the forward pass's xhat, not one that the rounding of mean / deviation went into: constant rows give dweight nothing."""
+    dt = TYPES[dtype]
+    x, dy, w = far_rows(D, dt), make("cpu", (10, D), dt, 5, 0.1, 0.7), make("cpu", (D,), torch.float32, 3, 1.0, 0.3)
+    (dx, dx_error), (dw, dw_error) = centred_backward(x, w, dy, 1e-5)
+    leaf, weight = x.to(cuda).requires_grad_(), w.to(cuda).requires_grad_()
+    got = torch.autograd.grad(ops.layer_norm(leaf, weight), (leaf, weight), dy.to(cuda))
+    near(got[0], dx, 0.0, dx_error)
+    near(got[1], dw, 0.0, dw_error)
+    for p in (0.0, 0.25):
+        branch = torch.zeros_like(x).to(cuda).requires_grad_()
+        y, z = ops.dropout_add_layer_norm(branch, leaf, weight, p=p, rng=(1, 2))
+        dbranch, dres, dweight = torch.autograd.grad((y, z), (branch, leaf, weight), (dy.to(cuda), torch.zeros_like(z)))
+        keep = O.keep_mask(10 * D, p, 1, 2).view(10, D).double() * O.drop_scale(p)
+        near(dbranch, dx * keep, 0.0, (dx_error + 2 * 2.0 ** -24 * dx.abs()) * keep)
+        near(dres, dx, 0.0, dx_error)
+        near(dweight, dw, 0.0, dw_error)
+
+
+@pytest.mark.parametrize("D", [64, 777, 2000, 9001])
+def test_layer_norm_backward_far_from_zero(cuda, D):
+    """f32 rows of mean 1000 and deviation 0.01, and of mean 4096 and deviation 1: forward and backward."""
+    x = torch.cat([make("cpu", (200, D), torch.float32, 1, 1000.0, 0.01), make("cpu", (200, D), torch.float32, 2, -4096.0, 1.0)])
+    dy, w = make("cpu", (400, D), torch.float32, 5, 0.1, 0.7), make("cpu", (D,), torch.float32, 3, 1.0, 0.3)
+    (dx, dx_error), (dw, dw_error) = centred_backward(x, w, dy, 1e-5)
+    leaf, weight = x.to(cuda).requires_grad_(), w.to(cuda).requires_grad_()
+    got = torch.autograd.grad(ops.layer_norm(leaf, weight), (leaf, weight), dy.to(cuda))
+    near(got[0], dx, 0.0, dx_error)
+    near(got[1], dw, 0.0, dw_error)
+
+
+def test_layer_norm_statistics_at_the_entry_points(cuda):
+    """Both forms of the statistics: with `stats`, xhat is as exact as in y; with mean and rstd it carries half a step of the mean, and no more."""
+    l, (rows, D) = _hip.lib(), (6, 300)
+    x, dy = make(cuda, (rows, D), torch.float32, 1, 1000.0, 0.01), make(cuda, (rows, D), torch.float32, 2)
+    x[5] = 13730.0
+    y, dx, dw, stats = torch.empty_like(x), torch.empty_like(x), torch.empty(D, device=cuda), torch.empty(rows, 3, device=cuda)
+    nb = l.yp_layer_norm_bwd_workspace_bytes(rows, D, _hip.YP_F32)
+    ws = torch.empty(nb, dtype=torch.uint8, device=cuda)
+    _, mean, rstd, _ = O.layer_norm(x.cpu(), None, None, 1e-5)
+    one = torch.ones(D)
+    (want, error), (want_w, error_w) = centred_backward(x.cpu(), one, dy.cpu(), 1e-5)
+    step = 2.0 ** -24 * mean.abs() * rstd                                            # (the nearest number is half a step away: 2^-24 of it)
+    m1 = dy.cpu().double().abs().mean(-1, keepdim=True)
+    m2 = (dy.cpu().double() * O.layer_norm(x.cpu(), None, None, 1e-5)[3]).abs().mean(-1, keepdim=True)
+    xhat = O.layer_norm(x.cpu(), None, None, 1e-5)[3].abs()
+    for rest in (True, False):
+        how = dict(rows=rows, D=D, dtype=_hip.YP_F32, wdtype=_hip.YP_F32, eps=1e-5, x=x.data_ptr(), x_stride=D,
+                   **(dict(stats=stats.data_ptr()) if rest else dict(mean=stats.view(-1)[:rows].data_ptr(), rstd=stats.view(-1)[rows:].data_ptr())))
+        stats.fill_(7.0)
+        _hip.check(l.yp_layer_norm_fwd(C.byref(_hip.YpLayerNormDesc(y=y.data_ptr(), **how)), _hip.stream_ptr()))
+        nearest = (stats[:, 0] if rest else stats.view(-1)[:rows]).cpu().double()
+        assert bool(((nearest - mean.view(-1)).abs() <= 2.0 ** -24 * mean.view(-1).abs() * 1.001).all())
+        if rest:
+            assert bool(((nearest + stats[:, 2].cpu().double() - mean.view(-1)).abs() <= 2.0 ** -36 * mean.view(-1).abs()).all())
+        else:
+            assert bool((stats.view(-1)[2 * rows:] == 7.0).all())
+        _hip.check(l.yp_layer_norm_bwd(C.byref(_hip.YpLayerNormDesc(dy=dy.data_ptr(), dy_stride=D, dres=dx.data_ptr(), dweight=dw.data_ptr(), workspace=ws.data_ptr(),
+                                                                    workspace_bytes=nb, **how)), _hip.stream_ptr()))
+        s = 0.0 if rest else step
+        near(dx, want, 0.0, error + rstd * s * (m2 + xhat * m1 + 2 * s * m1))
+        near(dw, want_w, 0.0, error_w + (dy.cpu().double().abs() * s).sum(0))

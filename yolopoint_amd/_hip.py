@@ -58,7 +58,7 @@ class YpLayerNormDesc(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("x", "res", "weight", "bias", "z", "y", "mean", "rstd", "dy", "dz", "dres", "dx", "dweight", "dbias", "workspace", "rng")]
                 + [(n, C.c_int64) for n in ("rows", "x_stride", "res_stride", "dy_stride", "dz_stride")]
                 + [("seed", C.c_uint64), ("offset", C.c_uint64), ("workspace_bytes", C.c_size_t), ("p", C.c_double), ("eps", C.c_float)]
-                + [(n, C.c_int32) for n in ("D", "dtype", "wdtype")])
+                + [(n, C.c_int32) for n in ("D", "dtype", "wdtype")] + [("stats", C.c_void_p)])
 
 
 YP_POS_I32, YP_POS_I64, YP_POS_F32 = 0, 1, 2

@@ -15,6 +15,9 @@ template <int G> __device__ __forceinline__ int row_in_block() {
     return G ? threadIdx.x / G : 0;
 }
 
+// a value that is the same in the whole wave, on the scalar unit (it frees a register of each lane)
+__device__ __forceinline__ float of_wave(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+
 // whether a thread is the last of its row's lanes in its wave
 template <int G> __device__ __forceinline__ bool last_lane() { return ((threadIdx.x + 1) & (G && G < 64 ? G - 1 : 63)) == 0; }
 

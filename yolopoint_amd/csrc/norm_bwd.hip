@@ -6,7 +6,7 @@ namespace {
 
 struct LnBwd {
     const void *z, *dy, *dz, *weight;
-    const float *mean, *rstd;
+    const float *mean, *rstd, *rest;                // [rows] each, or with_rest: one behind the other in lines of three; rest is the means again without it
     void *dres, *dx;
     float* partial;                                 // [gridDim.x][2][D]: dy xhat | dy summed over a workgroup's rows
     int64_t rows, zs, dys, dzs;
@@ -15,10 +15,15 @@ struct LnBwd {
     unsigned long long seed, offset;
     const int64_t* rng;
     unsigned threshold;
-    float scale;
+    float scale, inv_width;                         // 1 / D (an argument: no register of the lanes)
+    bool with_rest;
 };
 
 // h = dy w, c1 = mean h, c2 = mean (h xhat);  dres = [dz +] rstd (h - c1 - xhat c2);  dx = kept ? dres scale : 0.
+// xhat is the forward pass's: z rstd + shift is one multiply-add, whose shift -mean rstd carries the rounding of the product and of the mean; `low` is what
+// those left (without it a constant f32 row of 13730 had xhat 0.04, and dweight and dx got terms that do not exist).  Where xhat is formed a second
+// time (TIGHT) it is formed without it, and the row's sums are moved instead.  One addition a value: nothing where HBM bounds, up to 4 % at odd 16-bit
+// widths with dropout, 6 - 8 % at those of more than 8192 features.
 // dweight / dbias: a thread owns the same columns of every row it meets, so it sums them in its registers; a workgroup of some 512 threads joins its rows
 // through LDS and writes one line of partial sums; ln_columns_kernel adds the lines in order (no atomics: two passes give the same bits).
 // E = 16 (rows that 16 waves of 8 features a thread do not hold): no registers are left for the next row, nor for the weights, which wait in LDS (as
@@ -30,7 +35,7 @@ struct LnBwd {
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a) {
     constexpr int N = Vec<T>::N, NC = E / N;
-    constexpr bool TIGHT = E > 8;
+    constexpr bool TIGHT = E > 8, SCALAR = G == 0 && sizeof(T) == 2;       // SCALAR: a row's numbers wait on the scalar unit (fp32 rows lose by it)
     constexpr bool EARLY = !TIGHT && !(sizeof(T) == 4 && RES && DROP);     // the next row is on its way while this one is worked on, where registers are left
     __shared__ float2 sh[2][16];
     extern __shared__ float lds[];                  // TIGHT: the weights; then the space in which a workgroup's rows join
@@ -39,7 +44,6 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
     // threads of a row, rows of the workgroup, this thread's place
     const int threads = G ? G : a.waves * 64, each = G ? 512 / G : a.each;
     const int sub = G ? row_in_block<G>() : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) / a.waves), t = G ? threadIdx.x % G : threadIdx.x - sub * threads;
-    const float inv_d = 1.0f / (float)a.D;
     const Drop d = drop_state(a.seed, a.offset, a.rng, a.threshold, a.scale);
     int c[NC];
 #pragma unroll
@@ -48,7 +52,7 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
     // stores nothing)
     const int64_t first = (int64_t)blockIdx.x * each + sub, step = (int64_t)gridDim.x * each, end = G ? a.rows : (a.rows + each - 1) / each * each;
     Vec<T> nv[NC], ng[NC], ne[NC];
-    float nmean, nrstd;
+    float nmean, nrstd, nrest;
     int64_t at = min(first, a.rows - 1);
     const T *pz = z + at * a.zs, *pg = dy + at * a.dys, *pe = RES ? dz + at * a.dzs : nullptr;
     auto fetch = [&]() {
@@ -58,8 +62,10 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
             ng[k] = fetch_vec<T, TAIL>(pg, c[k], a.D);
             if constexpr (RES) ne[k] = fetch_vec<T, TAIL>(pe, c[k], a.D);
         }
-        nmean = a.mean[at];
-        nrstd = a.rstd[at];
+        const int64_t line = a.with_rest ? at * 3 : at;
+        nmean = a.mean[line];
+        nrstd = a.rstd[line];
+        nrest = a.rest[line];
     };
     if constexpr (EARLY) fetch();
     float w[TIGHT ? 1 : NC][N], dw[NC][N], db[NC][N];
@@ -101,7 +107,8 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
             if constexpr (RES) e[k] = settle<T, TAIL>(ne[k], c[k], a.D);
             if (!real) g[k] = Vec<T>{};
         }
-        const float rstd = nrstd, shift = -nmean * rstd;
+        float rstd = nrstd, shift = -nmean * rstd, low = fmaf(a.with_rest ? -nrest : 0.f, rstd, -fmaf(nmean, rstd, shift));
+        if constexpr (SCALAR) { rstd = of_wave(rstd); shift = of_wave(shift); low = of_wave(low); }
         if (row + step < end) {
             const int64_t next = min(row + step, a.rows - 1);
             pz += (next - at) * a.zs;
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
             weights(k, wk);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float gj = (float)g[k].e[j], xh = fmaf((float)v[k].e[j], rstd, sk);       // (gj is 0 behind the row's end)
+                const float gj = (float)g[k].e[j], xh = fmaf((float)v[k].e[j], rstd, sk) + low;  // (gj is 0 behind the row's end)
                 const float h = gj * wk[j];
                 dw[k][j] = fmaf(gj, xh, dw[k][j]);
                 db[k][j] += gj;
@@ -132,7 +139,9 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
         }
         row_sum2<G>(s1, s2, sh[slot], sub * a.waves, a.waves);
         slot ^= 1;
-        const float c1 = s1 * inv_d, c2 = s2 * inv_d;
+        float c1 = s1 * a.inv_width, c2 = s2 * a.inv_width;
+        if constexpr (TIGHT) c1 = fmaf(low, c2, c1);           // (where xhat is formed again, it is formed without its low part)
+        if constexpr (SCALAR) { c1 = of_wave(c1); c2 = of_wave(c2); }
         if (!real) continue;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -142,7 +151,7 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
             weights(k, wk);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float xh = fmaf((float)v[k].e[j], rstd, sk);
+                const float xh = TIGHT ? fmaf((float)v[k].e[j], rstd, sk) : fmaf((float)v[k].e[j], rstd, sk) + low;
                 const float h = (float)g[k].e[j] * wk[j];
                 const float s = fmaf(-xh, c2, h - c1);
                 if constexpr (RES) o[j] = fmaf(rstd, s, (float)e[k].e[j]);
@@ -318,15 +327,17 @@ extern "C" int yp_layer_norm_bwd(const YpLayerNormDesc* d, void* stream) {
         LnBwd a{};
         YP_REQUIRE(drop_parameters(d->p, &a.threshold, &a.scale), "yp_layer_norm_bwd: a dropout rate of %g", d->p);
         const bool res = d->dz != nullptr, drop = a.threshold != 0;
-        YP_REQUIRE(d->x && d->dy && d->mean && d->rstd && d->dres && (!drop || d->dx), "yp_layer_norm_bwd: a buffer is missing");
+        YP_REQUIRE(d->x && d->dy && (d->stats || (d->mean && d->rstd)) && d->dres && (!drop || d->dx), "yp_layer_norm_bwd: a buffer is missing");
         YP_REQUIRE(d->x_stride >= 0 && d->dy_stride >= 0 && d->dz_stride >= 0, "yp_layer_norm_bwd: negative stride");
         if (sums && (d->workspace == nullptr || d->workspace_bytes < yp_layer_norm_bwd_workspace_bytes(d->rows, d->D, d->dtype))) {
             yp_set_error("yp_layer_norm_bwd: workspace of %zu bytes, %zu needed", d->workspace_bytes, yp_layer_norm_bwd_workspace_bytes(d->rows, d->D, d->dtype));
             return YP_ERR_WORKSPACE;
         }
-        a.z = d->x; a.dy = d->dy; a.dz = d->dz; a.weight = d->weight; a.mean = d->mean; a.rstd = d->rstd; a.dres = d->dres; a.dx = d->dx;
+        a.z = d->x; a.dy = d->dy; a.dz = d->dz; a.weight = d->weight; a.with_rest = d->stats != nullptr;
+        a.mean = a.with_rest ? d->stats : d->mean; a.rstd = a.with_rest ? d->stats + 1 : d->rstd; a.rest = a.with_rest ? d->stats + 2 : d->mean;
+        a.dres = d->dres; a.dx = d->dx;
         a.partial = sums ? (float*)d->workspace : nullptr;
-        a.rows = d->rows; a.zs = d->x_stride; a.dys = d->dy_stride; a.dzs = d->dz_stride; a.D = d->D; a.w32 = d->wdtype == YP_F32;
+        a.rows = d->rows; a.zs = d->x_stride; a.dys = d->dy_stride; a.dzs = d->dz_stride; a.D = d->D; a.inv_width = 1.0f / (float)d->D; a.w32 = d->wdtype == YP_F32;
         a.seed = d->seed; a.offset = d->offset; a.rng = d->rng;
         YP_CHECK_HIP(d->dtype == YP_F16 ? ln_bwd_launch<_Float16>(a, res, drop, &lines, st) : d->dtype == YP_BF16 ? ln_bwd_launch<__bf16>(a, res, drop, &lines, st)
                                                                                              : ln_bwd_launch<float>(a, res, drop, &lines, st));

@@ -175,7 +175,7 @@ void check_drop(const char* what, const Tensor& x, double p, const MaybeTensor& 
 
 at::ScalarType weight_type(const Tensor& w, const Tensor& b) { return w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat; }
 
-struct NormResult { Tensor y, z, stats; };                 // stats: fp32 [2, rows], mean | 1 / deviation
+struct NormResult { Tensor y, z, stats; };                 // stats: fp32 [rows, 3], mean | 1 / deviation | what the mean's nearest fp32 number leaves
 
 NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias, double eps, const Dropping& drop, const Tensor& rng, bool keep) {
     const int64_t D = x.size(-1), rows = x.numel() / D;
@@ -193,9 +193,8 @@ NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& w
         d.z = r.z.data_ptr();
     }
     if (keep) {
-        r.stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
-        d.mean = (float*)r.stats.data_ptr();
-        d.rstd = d.mean + rows;
+        r.stats = at::empty({rows, 3}, x.options().dtype(at::kFloat));
+        d.stats = (float*)address(r.stats);
     }
     d.x = address(xr.t);
     d.x_stride = xr.stride;
@@ -264,8 +263,7 @@ struct NormBackward : Node {
             d.x_stride = zr.stride;
             d.dy = address(dyr.t);
             d.dy_stride = dyr.stride;
-            d.mean = (float*)address(stats_);
-            d.rstd = d.mean + rows;
+            d.stats = (float*)address(stats_);
             d.weight = address(w);
             d.dres = dres.data_ptr();
             d.dweight = address(dw);
