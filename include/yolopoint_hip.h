@@ -679,7 +679,8 @@ int yp_mnn_match(const float* d1, int N1, const float* d2, int N2, int D, float 
  *             nearest fp32 number leaves of the mean.
  *   backward  x = the z of the forward pass, mean / rstd (or stats) as it wrote them, dy = gradient of y, dz = gradient of z (NULL: none).  With
  *             stats the gradients are as exact as y on rows far from zero; without, they carry half a step of the mean, times rstd.
- *             dres = gradient of res (of x without a residual); dx = gradient of x, written where p > 0 only (it equals dres otherwise).
+ *             dres = gradient of res (of x without a residual); dx = gradient of x, written where p > 0 only (it equals dres otherwise).  Where dx
+ *             is not wanted: p = 0; where neither is: p = 0 and dres NULL.
  *             dweight, dbias in wdtype, each may be NULL; they need the workspace of yp_layer_norm_bwd_workspace_bytes (both NULL: none).
  *             Two passes over the same inputs give the same bits.
  *   dropout   rate p and the generator's state as in yp_dropout (element index = row * D + column).

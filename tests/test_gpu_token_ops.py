@@ -1093,3 +1093,48 @@ def test_layer_norm_statistics_at_the_entry_points(cuda):
         s = 0.0 if rest else step
         near(dx, want, 0.0, error + rstd * s * (m2 + xhat * m1 + 2 * s * m1))
         near(dw, want_w, 0.0, error_w + (dy.cpu().double().abs() * s).sum(0))
+
+
+# ------------------------------------------------------------------------------------------------------------------ what no one asked for
+def test_frozen_inputs_cost_the_backward_pass_no_tensors(cuda):
+    """Gradients of the rows are written where they are wanted only: each set of leaves gets the full pass's rows bit for bit, the weights' sums (over other
+    workgroups' parts, as the kernels differ) within their bound, and no more memory than its gradients."""
+    rows, D = 8192, 1000
+    x, r, dy, dz = (make(cuda, (rows, D), torch.bfloat16, i) for i in range(4))
+    w, b = make(cuda, (D,), torch.float32, 5), make(cuda, (D,), torch.float32, 6)
+    size = rows * D * 2
+    # beside the gradients: the partial sums, the weights' gradients, and what torch's allocator hands out unsplit (up to 1 MiB a buffer, five at the most)
+    sums = _hip.lib().yp_layer_norm_bwd_workspace_bytes(rows, D, _hip.YP_BF16) + 64 * D + (5 << 20)
+    assert sums < size                                                               # (a tensor too many shows)
+    for p in (0.0, 0.3):
+        full = None
+        for want in range(15, 0, -1):
+            leaves = [t.clone().requires_grad_(bool(want >> i & 1)) for i, t in enumerate((x, r, w, b))]
+            asked = [t for t in leaves if t.requires_grad]
+            for with_z in (True, False):
+                y, z = ops.dropout_add_layer_norm(*leaves, p=p, rng=(1, 2))
+                outs, grads = ((y, z), (dy, dz)) if with_z else ((y,), (dy,))
+                torch.cuda.synchronize()
+                before = torch.cuda.memory_allocated()
+                torch.cuda.reset_peak_memory_stats()
+                got = torch.autograd.grad(outs, asked, grads)
+                torch.cuda.synchronize()
+                peak = torch.cuda.max_memory_allocated() - before
+                # (x and the residual share one gradient where nothing is dropped; where something is, the residual's is written with x's)
+                tensors = (0, 2, 1, 2)[want & 3] if p else int(want & 3 != 0)
+                assert peak <= tensors * size + sums, (p, want, with_z, peak, tensors * size, sums)
+                if want == 15:
+                    full = full or {}
+                    full[with_z] = got
+                    _, dw, db = norm_backward_bound(z.detach().cpu(), w.cpu(), dy.cpu(), 1e-5)
+                for a, i in zip(got, [i for i in range(4) if want >> i & 1]):
+                    if i < 2:
+                        assert torch.equal(a, full[with_z][i])
+                    else:
+                        near(a, *(dw, db)[i - 2])
+    leaf = x.clone().requires_grad_()                                                # y unused: z's gradient goes through, in no pass over z
+    y, z = ops.dropout_add_layer_norm(r, leaf, w, b, p=0.3, rng=(1, 2))
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    assert torch.equal(torch.autograd.grad(z, leaf, dz)[0], dz)
+    assert torch.cuda.max_memory_allocated() - before < size

@@ -214,6 +214,13 @@ NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& w
     return r;
 }
 
+Tensor drop_launch(const Tensor& x, const Tensor& residual, const Dropping& drop, const Tensor& rng) {
+    const Tensor xc = dense(x), rc = dense(residual);
+    Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+    check(lib.dropout(address(xc), address(rc), y.data_ptr(), x.numel(), type_code(x.scalar_type()), drop.p, drop.seed, drop.offset, (const int64_t*)address(rng), stream_of(x)));
+    return y;
+}
+
 struct NormBackward : Node {
     SavedVariable z, weight, stats, rng;                   // z: what was normalised (the input itself without a residual)
     Dropping drop;
@@ -240,19 +247,29 @@ struct NormBackward : Node {
         {
             at::AutoDispatchBelowADInplaceOrView below;
             const c10::DeviceGuard guard(z_.device());
-            if (!dy.defined()) dy = at::zeros_like(dz);
+            const bool drops = drop.any(), need_x = task_should_compute_output(0), need_res = fused && task_should_compute_output(1);
+            const bool need_w = task_should_compute_output(n - 2), need_b = task_should_compute_output(n - 1);
+            const auto options = z_.options().memory_format(at::MemoryFormat::Contiguous);
+            if (!dy.defined()) {                           // y was not used: the gradient of z goes on to its parts
+                if (need_res) out[1] = dz;
+                if (need_x) out[0] = drops ? drop_launch(dz, Tensor(), drop, rng_) : dz;
+                if (need_w) out[n - 2] = at::zeros({z_.size(-1)}, options.dtype(wtype));
+                if (need_b) out[n - 1] = at::zeros({z_.size(-1)}, options.dtype(wtype));
+                return once(std::move(out));
+            }
             const int64_t D = z_.size(-1), rows = z_.numel() / D;
             const Rows zr = rows_of(z_), dyr = rows_of(dy);
             Rows dzr;
             const Tensor w = dense(w_);
-            const auto options = z_.options().memory_format(at::MemoryFormat::Contiguous);
-            const Tensor dres = at::empty(z_.sizes(), options);
-            const bool drops = drop.any();
-            Tensor dx, dw, db, ws;
+            Tensor dres, dx, dw, db, ws;
             YpLayerNormDesc d{};
-            if (drops) { dx = at::empty(z_.sizes(), options); d.dx = dx.data_ptr(); }
-            if (task_should_compute_output(n - 2) && next_edge(n - 2).is_valid()) dw = at::empty({D}, options.dtype(wtype));
-            if (task_should_compute_output(n - 1) && next_edge(n - 1).is_valid()) db = at::empty({D}, options.dtype(wtype));
+            // (the branch's gradient is another tensor than the residual's only where elements were dropped; rows that no one asked for are not written)
+            const bool rows_wanted = need_res || need_x;
+            if (rows_wanted) { dres = at::empty(z_.sizes(), options); d.dres = address(dres); }
+            if (need_x && drops) { dx = at::empty(z_.sizes(), options); d.dx = address(dx); }
+            if (need_w) dw = at::empty({D}, options.dtype(wtype));
+            if (need_b) db = at::empty({D}, options.dtype(wtype));
+            if (!rows_wanted) dz = Tensor();
             if (dw.defined() || db.defined()) {            // (a workspace of its own in every call: streams and captured graphs share none)
                 d.workspace_bytes = lib.norm_workspace(rows, (int)D, type_code(z_.scalar_type()));
                 ws = at::empty({(int64_t)d.workspace_bytes}, options.dtype(at::kByte));
@@ -265,20 +282,21 @@ struct NormBackward : Node {
             d.dy_stride = dyr.stride;
             d.stats = (float*)address(stats_);
             d.weight = address(w);
-            d.dres = dres.data_ptr();
             d.dweight = address(dw);
             d.dbias = address(db);
             d.rows = rows;
             d.D = (int32_t)D;
             d.dtype = type_code(z_.scalar_type());
             d.wdtype = type_code(wtype);
-            d.p = drop.p;
-            d.seed = drop.seed;
-            d.offset = drop.offset;
-            d.rng = (const int64_t*)address(rng_);
+            if (dx.defined()) {
+                d.p = drop.p;
+                d.seed = drop.seed;
+                d.offset = drop.offset;
+                d.rng = (const int64_t*)address(rng_);
+            }
             check(lib.norm_bwd(&d, stream_of(z_)));
-            out[0] = drops ? dx : dres;
-            if (fused) out[1] = dres;
+            if (need_x) out[0] = drops ? dx : dres;
+            if (need_res) out[1] = dres;
             out[n - 2] = dw;
             out[n - 1] = db;
         }
@@ -343,13 +361,6 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const MaybeTe
 }
 
 // ---------------------------------------------------------------------------------------------------------------- dropout
-Tensor drop_launch(const Tensor& x, const Tensor& residual, const Dropping& drop, const Tensor& rng) {
-    const Tensor xc = dense(x), rc = dense(residual);
-    Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    check(lib.dropout(address(xc), address(rc), y.data_ptr(), x.numel(), type_code(x.scalar_type()), drop.p, drop.seed, drop.offset, (const int64_t*)address(rng), stream_of(x)));
-    return y;
-}
-
 struct DropoutBackward : Node {
     SavedVariable rng;
     Dropping drop;
