@@ -96,7 +96,7 @@ def self_launch(a, argv):
     """`python bench.py --gpus N` with N > 1 and no launcher around it (WORLD_SIZE unset): run `torch.distributed.run --nnodes=1
     --nproc-per-node N --master-addr 127.0.0.1 --master-port P bench.py <same arguments>` -- one rank per GPU, the form the reference is
     started in (`accelerate launch src/train.py`, README.md:76; train.py:38-46,174), as a child process that inherits stdout (rank 0's ONE JSON
-    line passes unchanged) and whose exit code this process returns: counting the GPUs initialises the runtime, and such a process must not be
+    line passes unchanged), gets the signals that this process is stopped with and whose exit code it returns: counting the GPUs initialises the runtime, and such a process must not be
     replaced by another program (exec is refused on the GPU machines).  Fails loudly when the box has fewer than N GPUs (never a silent N = 1 run)."""
     if not a.dry:
         have = torch.cuda.device_count() if torch.cuda.is_available() else 0
@@ -117,8 +117,20 @@ def self_launch(a, argv):
            "--master-port", port, os.path.abspath(__file__)] + list(argv)
     sys.stderr.write("bench.py: launching " + " ".join(cmd) + "\n")
     sys.stderr.flush()
+    import signal
     import subprocess
-    rc = subprocess.call(cmd)
+    child, stopped = None, []
+
+    def forward(number, frame):                   # what stops this process stops the ranks: they would hold the GPUs otherwise
+        stopped.append(number)
+        if child is not None and child.poll() is None:
+            child.send_signal(number)
+    for number in (signal.SIGTERM, signal.SIGINT, signal.SIGHUP):
+        signal.signal(number, forward)
+    child = subprocess.Popen(cmd)
+    if stopped:                                   # (between the handlers and here)
+        child.send_signal(stopped[-1])
+    rc = child.wait()
     sys.exit(rc if rc >= 0 else 128 - rc)
 
 

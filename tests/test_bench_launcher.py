@@ -6,9 +6,11 @@ which re-executes itself under torch.distributed.run).  `--backend gloo --dry` r
 of the real records with a stub step, so the rank plumbing is checked here without a GPU."""
 import json
 import os
+import signal
 import socket
 import subprocess
 import sys
+import time
 
 import pytest
 
@@ -66,3 +68,17 @@ def test_world_size_and_gpus_must_agree():
     env.update(WORLD_SIZE="1", RANK="0", LOCAL_RANK="0")
     r = subprocess.run([sys.executable, BENCH, "--gpus", "2", "--backend", "gloo", "--dry"], capture_output=True, text=True, timeout=300, env=env, cwd=ROOT)
     assert r.returncode != 0 and "WORLD_SIZE=1" in r.stderr and r.stdout.strip() == ""
+
+
+@pytest.mark.parametrize("number", [signal.SIGTERM, signal.SIGINT])
+def test_a_stopped_launcher_stops_its_ranks(number):
+    """`timeout` and schedulers signal the process they started: the ranks must not go on by themselves and print their record behind it."""
+    p = subprocess.Popen([sys.executable, BENCH, "--gpus", "2", "--backend", "gloo", "--dry", "--steps", "4", "--warmup", "1"], stdout=subprocess.PIPE, stderr=subprocess.PIPE,
+                         text=True, env=_env(), cwd=ROOT)
+    for line in p.stderr:
+        if "launching" in line:
+            break
+    time.sleep(0.3)
+    p.send_signal(number)
+    out, err = p.communicate(timeout=120)          # (until every process that holds the pipe has ended)
+    assert p.returncode != 0 and out.strip() == "", (p.returncode, out[:400])
