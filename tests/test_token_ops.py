@@ -224,3 +224,12 @@ def test_rotary_refuses_head_counts_past_32_bits():
                          (1 << 30, 0, 1 << 10, 1 << 20)):
         d = _hip.YpRotaryDesc(q=64, k=64, q_out=64, k_out=64, positions=64, inv_freq=64, B=B, T=T, Hq=Hq, Hk=Hk, D=2, R=2, axes=1, scale=1.0)
         assert l.yp_rotary(C.byref(d), None) == -1 and b"heads" in l.yp_last_error()
+
+
+def test_the_library_builds_without_torch():
+    """`make` for a C program: no torch, no Python headers."""
+    def commands(*more):
+        return subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "yolopoint_amd", "csrc"), *more, "all"], check=True, capture_output=True, text=True)
+    bare, full = commands("PYTHON=/bin/false"), commands()
+    assert "libyolopoint_hip.so" in bare.stdout and "token_autograd" not in bare.stdout and "Traceback" not in bare.stderr
+    assert "libyolopoint_hip.so" in full.stdout and "token_autograd.cpp" in full.stdout
