@@ -233,3 +233,11 @@ def test_the_library_builds_without_torch():
     bare, full = commands("PYTHON=/bin/false"), commands()
     assert "libyolopoint_hip.so" in bare.stdout and "token_autograd" not in bare.stdout and "Traceback" not in bare.stderr
     assert "libyolopoint_hip.so" in full.stdout and "token_autograd.cpp" in full.stdout
+
+
+def test_build_compiles_where_a_library_is_there(monkeypatch):
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: calls.append(cmd))
+    entry.build()
+    assert calls[0][0] == "make" and "-B" in calls[0]
