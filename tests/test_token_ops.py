@@ -241,3 +241,11 @@ def test_build_compiles_where_a_library_is_there(monkeypatch):
     monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: calls.append(cmd))
     entry.build()
     assert calls[0][0] == "make" and "-B" in calls[0]
+
+
+def test_no_build_of_the_kernels_has_packed_fp32():
+    """Every compiled object, of the library and of the sanitizer's, leaves those instructions out."""
+    for goal in ("all", "asan"):
+        out = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "yolopoint_amd", "csrc"), goal], check=True, capture_output=True, text=True).stdout
+        lines = [l for l in out.splitlines() if ".hip -o" in l]
+        assert len(lines) >= 14 and all("-Xclang -target-feature -Xclang -packed-fp32-ops" in l for l in lines), goal
