@@ -1138,3 +1138,42 @@ def test_frozen_inputs_cost_the_backward_pass_no_tensors(cuda):
     torch.cuda.reset_peak_memory_stats()
     assert torch.equal(torch.autograd.grad(z, leaf, dz)[0], dz)
     assert torch.cuda.max_memory_allocated() - before < size
+
+
+FIRST_CALL = """
+import torch
+from yolopoint_amd.utils import token_ops as ops
+cuda, D = torch.device("cuda:0"), 16000
+g = torch.Generator().manual_seed(1)
+x0, dy, w0 = (torch.randn(s, generator=g).half().to(cuda) for s in ((7, D), (7, D), (D,)))
+st = torch.cuda.Stream()
+st.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(st):
+    x, w = x0.clone().requires_grad_(), w0.clone().requires_grad_()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=st):
+    y = ops.layer_norm(x, w)
+    out = (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+for i in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    ex, ew = x.detach().clone().requires_grad_(), w0.clone().requires_grad_()
+    ey = ops.layer_norm(ex, ew)
+    assert all(torch.equal(p, q) for p, q in zip(out, (ey, *torch.autograd.grad(ey, (ex, ew), dy)))), i
+    with torch.no_grad():
+        x.mul_(0.5)
+torch.cuda.synchronize()
+print("captured first call: ok")
+"""
+
+
+def test_captured_first_call_in_a_process_of_its_own(cuda):
+    """The captured call is the process's first of these kernels, so that what the launch asks the runtime for (a larger LDS limit, the occupancy) is asked
+    inside the capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=100, cwd=root)
+    assert r.returncode == 0 and "captured first call: ok" in r.stdout, r.stderr[-2000:]
