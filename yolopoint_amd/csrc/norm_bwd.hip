@@ -22,7 +22,7 @@ struct LnBwd {
 // h = dy w, c1 = mean h, c2 = mean (h xhat);  dres = [dz +] rstd (h - c1 - xhat c2);  dx = kept ? dres scale : 0.
 // xhat is the forward pass's: z rstd + shift is one multiply-add, whose shift -mean rstd carries the rounding of the product and of the mean; `low` is what
 // those left (without it a constant f32 row of 13730 had xhat 0.04, and dweight and dx got terms that do not exist).  Where xhat is formed a second
-// time (TIGHT) it is formed without it, and the row's sums are moved instead.  One addition a value: nothing where HBM bounds, up to 4 % at odd 16-bit
+// time (TIGHT) it is formed without it, and the row's sums are moved instead.  One addition a value: nothing where HBM bounds, 3 - 5 % at odd 16-bit
 // widths with dropout, 6 - 8 % at those of more than 8192 features.
 // dweight / dbias: a thread owns the same columns of every row it meets, so it sums them in its registers; a workgroup of some 512 threads joins its rows
 // through LDS and writes one line of partial sums; ln_columns_kernel adds the lines in order (no atomics: two passes give the same bits).
@@ -35,7 +35,7 @@ struct LnBwd {
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a) {
     constexpr int N = Vec<T>::N, NC = E / N;
-    constexpr bool TIGHT = E > 8, SCALAR = G == 0 && sizeof(T) == 2;       // SCALAR: a row's numbers wait on the scalar unit (fp32 rows lose by it)
+    constexpr bool TIGHT = E > 8, SCALAR = TIGHT && sizeof(T) == 2;       // SCALAR: a row's numbers wait on the scalar unit (fp32 rows and narrower ones lose by it)
     constexpr bool EARLY = !TIGHT && !(sizeof(T) == 4 && RES && DROP);     // the next row is on its way while this one is worked on, where registers are left
     __shared__ float2 sh[2][16];
     extern __shared__ float lds[];                  // TIGHT: the weights; then the space in which a workgroup's rows join
