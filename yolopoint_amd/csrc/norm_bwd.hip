@@ -159,7 +159,7 @@ __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a
             }
             Vec<T> ov;
             if constexpr (DROP) {
-                drop_only<T, TAIL != WHOLE, G == 0 || G == 64>(d, (unsigned long long)row * a.D + c[k], o, ov, last_lane<G>(), a.D - c[k]);
+                drop_only<T, TAIL != WHOLE, G == 0 || G == 64, sizeof(T) == 2 && !(TIGHT && TAIL != WHOLE)>(d, (unsigned long long)row * a.D + c[k], o, ov, last_lane<G>(), a.D - c[k]);
                 store_vec<T, TAIL>(dx + row * a.D, c[k], a.D, ov);
             }
             store_vec<T, TAIL>(dres + row * a.D, c[k], a.D, to_vec<T>(o));

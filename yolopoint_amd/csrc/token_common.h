@@ -243,15 +243,16 @@ __device__ __forceinline__ void drop_add(const Drop& d, unsigned long long i, co
     out = to_vec<T>(s);
 }
 
-// out = kept ? v * scale : 0.  The generator's products as 64-bit multiply-adds for eight 16-bit elements, which its instructions bound (backward of
-// 31956 x 2100 bf16 210 us against 232, 86369 x 777 168 against 178, 13421 x 5000 132 against 149; at worst 16372 x 4099 236 against 231; dropout of
-// 8.4 M elements 8.4 against 8.9); as halves for four fp32 elements, where the pairs of registers cost more (8186 x 4099: 148 against 157) than the
-// products, and in drop_add (forward of 16372 x 4099 bf16: 159 against 187).
-template <typename T, bool STRADDLE = false, bool WAVE = false>
+// out = kept ? v * scale : 0.  MAD: the generator's products as 64-bit multiply-adds, for eight 16-bit elements, which its instructions bound (backward of
+// 31956 x 2100 bf16 224 us against 239, 86369 x 777 192 against 203, 13421 x 5000 132 against 150; at worst 16372 x 4099 245 against 235; dropout of
+// 8.4 M elements 8.4 against 8.9).  As halves where the pairs of registers cost more than the products: four fp32 elements (8186 x 4099: 148 against
+// 157), odd rows of more than 8192 features (5436 x 12345 bf16: 257 against 280, 8201 features 279 against 308), and drop_add (forward of 16372 x 4099
+// bf16: 159 against 187).
+template <typename T, bool STRADDLE = false, bool WAVE = false, bool MAD = sizeof(T) == 2>
 __device__ __forceinline__ void drop_only(const Drop& d, unsigned long long i, const float (&v)[Vec<T>::N], Vec<T>& out, bool edge = false, int left = 0) {
     constexpr int N = Vec<T>::N;
     unsigned w[N / 2];
-    drop_bits<N, STRADDLE, WAVE, N == 8>(d, i, edge, left, w);
+    drop_bits<N, STRADDLE, WAVE, MAD>(d, i, edge, left, w);
     float s[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = drop_kept<N>(d, w, j) ? v[j] * d.scale : 0.f;
