@@ -29,8 +29,8 @@ struct LnFwd {
 // 143 us against 170.)
 // The next row is on its way while this one is worked on (the first before the weights are read): its registers are not touched before its turn, or the
 // wait for them would stand right behind the loads.
-// Measured, 128 MiB a tensor: 44 - 60 us for widths 16 .. 16384 (4.5 - 6.2 TB/s), with residual and dropout 100 - 130 us (4.1 - 5.4; a large copy: 5.2 - 5.4);
-// widths just over a border with dropout are bound by their instructions (bf16 4100: 142 us, 4099: 158).
+// Measured, 128 MiB a tensor, with the statistics: 44 - 67 us for widths 16 .. 16384 (4.0 - 6.2 TB/s), with residual and dropout 100 - 130 us (4.1 - 5.4; a
+// large copy: 5.2 - 5.4); widths just over a border with dropout are bound by their instructions (bf16 4100: 142 us, 4099: 158, 12345: 160).
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 256 : 1024, G == 0 && sizeof(T) == 2 ? 5 : 1) void ln_fwd_kernel(const LnFwd a) {
     constexpr int N = Vec<T>::N, NC = E / N, ROWS = G ? 256 / G : 1;
@@ -98,8 +98,8 @@ __global__ __launch_bounds__(G ? 256 : 1024, G == 0 && sizeof(T) == 2 ? 5 : 1) v
         float var = fmaf(-delta, delta, s2 * a.inv_width);
         var = var < 0.f ? 0.f : var;                // (not fmaxf: a NaN stays one)
         const float rstd = rsqrtf(var + a.eps), shift = -delta * rstd;
-        // (Rows of a wave or less: one store by as many lanes, three take 70 us against 63 for bf16 rows of 16.  Wider ones: one lane without a branch
-        // inside, for its sake they lose up to 172 us against 125 at 2100 features with dropout; a rest that has no place is written under the mean.)
+        // (Rows of a wave or less: one store by as many lanes, three take 70 us against 63 for bf16 rows of 16.  Wider ones: three by one lane, the other
+        // way takes 138 us against 125 at 2100 features with dropout, and a branch for each 172; a rest that has no place is written under the mean.)
         const float nearest = mean + delta, rest = delta - (nearest - mean);            // (exact: |delta| is some steps of the mean)
         if constexpr (G != 0) {
             if (t < a.parts) a.stats[row * a.line + (t == 1 ? a.rstd : t)] = t == 0 ? nearest : t == 1 ? rstd : rest;

@@ -29,9 +29,10 @@ struct LnBwd {
 // E = 16 (rows that 16 waves of 8 features a thread do not hold): no registers are left for the next row, nor for the weights, which wait in LDS (as
 // 16-byte pieces: no bank twice); between the sums and the result the row waits in the type it was loaded in, and xhat and h are formed again (the
 // empty asm keeps the compiler from holding them in fp32 instead); one chunk after the other, so that only one's random numbers are live.
-// Measured, 128 MiB a tensor: 80 - 104 us for widths 16 .. 16384 (3.9 - 5.1 TB/s over the two tensors read and one written), through residual and dropout
-// 130 - 156 us (4.3 - 5.1 over five); odd bf16 widths with dropout are bound by their instructions (777: 168, 2100: 210, 4099: 236 us), fp32 rows of more than 8192 features by
-// registers that do not suffice (16384: 204 us).
+// Measured, 128 MiB a tensor: 79 - 106 us for widths 16 .. 16384 (3.8 - 5.1 TB/s over the two tensors read and one written; odd 16-bit widths over 4096: 115 -
+// 135), through residual and dropout 129 - 164 us (4.1 - 5.2 over five); odd bf16 widths with dropout are bound by their instructions (777: 170, 2100: 217,
+// 4099: 244, 12345: 257 us), rows of more than 8192 features by registers that do not suffice: all their fp32 kernels spill 12 - 55 (16384 with dropout:
+// 204 us), the 16-bit ones with dropout up to 14.
 template <typename T, int G, int E, bool RES, bool DROP, Tail TAIL>
 __global__ __launch_bounds__(G ? 512 : 1024, 4) void ln_bwd_kernel(const LnBwd a) {
     constexpr int N = Vec<T>::N, NC = E / N;
