@@ -46,6 +46,9 @@ enum { YP_F16 = 0, YP_BF16 = 1, YP_F32 = 2,
 enum { YP_ACT_NONE = 0, YP_ACT_SILU = 1 };
 
 const char* yp_last_error(void);
+/* The interface's version: it rises where a descriptor grows (at its end), so that a program can tell before its first call that the library reads more of
+ * a descriptor than the header it was compiled with has: yp_version() > YP_VERSION.  101: YpLayerNormDesc.stats */
+#define YP_VERSION 101
 int yp_version(void);
 /* number of HIP devices visible, 0 when none (never fails, usable on a CPU-only host) */
 int yp_device_count(void);

@@ -249,3 +249,13 @@ def test_no_build_of_the_kernels_has_packed_fp32():
         out = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "yolopoint_amd", "csrc"), goal], check=True, capture_output=True, text=True).stdout
         lines = [l for l in out.splitlines() if ".hip -o" in l]
         assert len(lines) >= 14 and all("-Xclang -target-feature -Xclang -packed-fp32-ops" in l for l in lines), goal
+
+
+def test_the_version_rose_with_the_descriptor(tmp_path):
+    """A program built against an earlier header passes a shorter YpLayerNormDesc: it can tell by the version."""
+    src = tmp_path / "version.c"
+    src.write_text('#include "yolopoint_hip.h"\n#include <stdio.h>\nint main(void) { printf("%d %zu %zu", YP_VERSION, offsetof(YpLayerNormDesc, stats), sizeof(YpLayerNormDesc)); return 0; }\n')
+    exe = tmp_path / "version"
+    subprocess.run(["gcc", "-include", "stddef.h", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    version, offset, size = (int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split())
+    assert _hip.lib().yp_version() == version >= 101 and offset + C.sizeof(C.c_void_p) == size

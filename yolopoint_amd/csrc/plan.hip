@@ -21,7 +21,7 @@ void yp_set_error(const char* fmt, ...) {
 }
 
 extern "C" const char* yp_last_error(void) { return g_err; }
-extern "C" int yp_version(void) { return 100; }
+extern "C" int yp_version(void) { return YP_VERSION; }
 extern "C" int yp_device_count(void) {
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess) { (void)hipGetLastError(); return 0; }
